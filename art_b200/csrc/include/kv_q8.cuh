@@ -1,0 +1,72 @@
+// Numbers of a cache of keys and values held in 8 bits.
+//
+// Codes [blocks, Hkv, block_size, hd], e4m3 or int8, and one fp32 scale per block and kv head [blocks, Hkv]: value = code *
+// scale.  The codes of a block and head are block_size * hd bytes in a row.  Scales are powers of two, so that x / scale is
+// exact in fp32 and every code is one rounding of its value; the least such scale costs up to one bit of the 7 that int8 has
+// and nothing of e4m3's 4, whose spacing goes with the value.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "ptx_sm100.cuh"
+
+namespace artb {
+
+enum Q8Kind : int { Q8_E4M3 = 0, Q8_INT8 = 1 };
+
+constexpr int Q8_LEAST_EXP = -126;       // the smallest scale is a normal fp32 number
+
+// Index checks of these kernels are always on: slots and block tables come from memory, and a compare costs nothing beside
+// the access it guards.
+__device__ __forceinline__ bool q8_index_ok(long long i, long long n, int* status) {
+  if (i < 0 || i >= n) {
+    if (status) atomicMax(status, ST_BOUNDS);
+    return false;
+  }
+  return true;
+}
+
+__device__ __forceinline__ float q8_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
+
+// Exponent of the least power of two s with amax <= MAX * s (448 = 1.75 * 2^8, 127 = 1.984375 * 2^6), from the bits of a
+// finite fp32 amax.  A subnormal amax is below every scale's range.
+template <int KIND>
+__device__ __forceinline__ int q8_exponent(uint32_t amax_bits) {
+  constexpr int TOP = KIND == Q8_E4M3 ? 8 : 6;
+  constexpr uint32_t FRACTION = KIND == Q8_E4M3 ? 0x600000u : 0x7e0000u;
+  const int e = static_cast<int>(amax_bits >> 23) - 127 - TOP + ((amax_bits & 0x7fffffu) > FRACTION);
+  return e < Q8_LEAST_EXP ? Q8_LEAST_EXP : e;
+}
+
+// Four values, already divided by their scale, to four codes: nearest, ties to even.
+template <int KIND>
+__device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float d) {
+  if (KIND == Q8_E4M3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+  const uint32_t x = __float2int_rn(a), y = __float2int_rn(b), z = __float2int_rn(c), w = __float2int_rn(d);
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
+// Four codes to floats.
+template <int KIND>
+__device__ __forceinline__ void q8_decode4(uint32_t w, float (&f)[4]) {
+  if (KIND == Q8_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * i)), __NV_E4M3);
+      const float2 v = __half22float2(__half2(h));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  }
+}
+
+}  // namespace artb

@@ -1,0 +1,169 @@
+"""Front-ends of a paged cache of keys and values held in 8 bits: write, read-back, decode attention.
+
+A cache is four tensors of a layer: codes ``k_cache`` and ``v_cache`` ``[blocks, Hkv, block_size, hd]`` (``torch.float8_e4m3fn``
+or ``torch.int8``) and scales ``k_scale`` and ``v_scale`` ``[blocks, Hkv]`` fp32.  A value is its code times the scale of its
+block and kv head; scales are powers of two (csrc/include/kv_q8.cuh).  A zeroed cache is an empty one.
+
+Half the bytes of the bf16 cache (:mod:`.paged`), which is what bounds both the number of sequences that run at a time and decode
+attention.  ``e4m3`` keeps 4 significant bits of every value, ``int8`` an absolute step of less than 1/63 of the largest value in
+the block and head.  The reference has the choice as ``engine_args.kv_cache_dtype`` (src/art/dev/engine.py:24) of the engine it
+serves through.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from . import _lib
+
+vp, ci, cl = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+_sigs = {
+    "artb_kv_write_q8": [vp, ci, ci, ci, vp, vp, vp, vp, vp, ci, ci, ci, ci, cl, ci, vp, vp],
+    "artb_kv_rows_q8": [vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, ci, cl, ci, vp, vp],
+    "artb_paged_decode_q8": [vp, ci, vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, vp, ci, vp, cl, ci, vp, vp],
+    "artb_paged_decode_q8_bytes": [ci, ci, ci, ci],
+}
+_bound: dict[str, object] = {}
+
+KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+HEAD_DIMS = (32, 64, 128)
+
+
+def _f(name: str):
+    fn = _bound.get(name)
+    if fn is None:
+        fn = getattr(_lib.kernels(), name)
+        fn.argtypes = _sigs[name]
+        fn.restype = ci
+        _bound[name] = fn
+    return fn
+
+
+def check_geometry(dtype: torch.dtype, block_size: int, hd: int) -> None:
+    """Refuses what the kernels do not cover."""
+    if dtype not in KINDS:
+        raise ValueError(f"a cache of {dtype}: codes are float8_e4m3fn or int8")
+    if block_size < 16 or block_size % 16:
+        raise ValueError(f"blocks of {block_size} tokens: a cache in 8 bits has blocks of a multiple of 16")
+    if hd not in HEAD_DIMS:
+        raise ValueError(f"head dim {hd}: a cache in 8 bits takes {', '.join(map(str, HEAD_DIMS))}")
+
+
+def _check_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
+    """(blocks, Hkv, block_size, hd) of a cache that is one."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} {v_cache.dtype} differ "
+                         "or are not [blocks, Hkv, block_size, hd]")
+    nb, hkv, bs, hd = k_cache.shape
+    check_geometry(k_cache.dtype, bs, hd)
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s.shape != (nb, hkv) or s.dtype != torch.float32 or not s.is_contiguous():
+            raise ValueError(f"{name} must be contiguous fp32 [{nb}, {hkv}]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache and v_cache must be contiguous")
+    return nb, hkv, bs, hd
+
+
+def _check_rows(name: str, x: torch.Tensor, cols: tuple, width: int) -> None:
+    """``x`` [rows, ld] bf16 that holds ``width`` columns from each of ``cols`` on, in pieces of 16 bytes."""
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{name} must be bf16 [rows, columns] with unit inner stride")
+    if any(c < 0 or c % 8 or c + width > x.shape[1] for c in cols):
+        raise ValueError(f"{name} [{x.shape[0]}, {x.shape[1]}] does not hold {width} columns at {cols}, multiples of 8")
+    if x.shape[0] > 1 and x.stride(0) % 8 or x.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must begin on 16 bytes")
+
+
+def _check_index(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}]")
+
+
+def _device(*tensors: torch.Tensor) -> torch.device:
+    dev = tensors[0].device
+    if dev.type != "cuda" or any(t.device != dev for t in tensors):
+        raise ValueError(f"tensors of one CUDA device are needed: {', '.join(sorted({str(t.device) for t in tensors}))}")
+    return dev
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """On the current stream of ``dev``, whichever device is current."""
+    what = name.removeprefix("artb_")
+    if dev.index == torch.cuda.current_device():
+        _lib.check_rc(_f(name)(*args, _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr()), what)
+    else:
+        with torch.cuda.device(dev):
+            _lib.check_rc(_f(name)(*args, _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr()), what)
+
+
+def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Quantises the keys and values of the rows of ``qkv`` (bf16 [M, >= ...], columns ``k_col`` and ``v_col`` on) into the cache.
+    ``slot`` int32 [M]: block * block_size + place, negative: the row is not written.  The rows of a block stand next to each other
+    in the order of their places, and a slot occurs once.
+
+    The scale of a block and head is the least power of two that takes the largest value written to it into the range of the
+    codes.  A row at a block's first place starts the block anew.  Rows at later places can only raise the scale, and then what
+    the block holds already is rounded once more.  A value that is not finite makes the scale NaN until the block starts anew."""
+    nb, hkv, bs, hd = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    _check_rows("qkv", qkv, (k_col, v_col), hkv * hd)
+    _check_index("slot", slot, qkv.shape[0])
+    dev = _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
+    _launch(dev, "artb_kv_write_q8", _lib.ptr(qkv), qkv.stride(0), k_col, v_col, _lib.ptr(slot), _lib.ptr(k_cache), _lib.ptr(v_cache),
+            _lib.ptr(k_scale), _lib.ptr(v_scale), qkv.shape[0], hkv, hd, bs, nb, KINDS[k_cache.dtype])
+
+
+def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot: torch.Tensor,
+               dst: torch.Tensor, k_col: int, v_col: int) -> None:
+    """The cached keys and values at ``slot`` (int32 [n]) as bf16 into the k and v columns of ``dst[:n]``; zeros where negative."""
+    nb, hkv, bs, hd = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    _check_rows("dst", dst, (k_col, v_col), hkv * hd)
+    if abs(k_col - v_col) < hkv * hd or (dst.shape[0] > 1 and dst.stride(0) < max(k_col, v_col) + hkv * hd):
+        raise ValueError("the columns of keys and values, or the rows of dst, overlap")
+    n = slot.numel()
+    _check_index("slot", slot, n)
+    if n > dst.shape[0]:
+        raise ValueError(f"{n} slots for {dst.shape[0]} rows")
+    dev = _device(dst, slot, k_cache, v_cache, k_scale, v_scale)
+    _launch(dev, "artb_kv_rows_q8", _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(slot), n,
+            _lib.ptr(dst), dst.stride(0), k_col, v_col, hkv, hd, bs, nb, KINDS[k_cache.dtype])
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_bytes(n: int, Hq: int, Hkv: int, hd: int, device: int | None) -> int:
+    with torch.cuda.device(device):
+        return _f("artb_paged_decode_q8_bytes")(n, Hq, Hkv, hd)
+
+
+def decode_q8_workspace(n: int, Hq: int, Hkv: int, hd: int, device) -> torch.Tensor:
+    """Workspace of :func:`paged_decode_q8` for up to ``n`` sequences; one call at a time may use it."""
+    return torch.zeros(_decode_bytes(n, Hq, Hkv, hd, torch.device(device).index), dtype=torch.uint8, device=device)
+
+
+def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    block_table: torch.Tensor, ctx_len: torch.Tensor, Hq: int, Hkv: int, hd: int, out: torch.Tensor,
+                    ws: torch.Tensor) -> torch.Tensor:
+    """Attention of one token per sequence over the first ``ctx_len`` cached tokens: q bf16 [n, >= Hq*hd] (row stride arbitrary),
+    ``block_table`` int32 [n, width], ``ctx_len`` int32 [n] (0: the row becomes zeros); out bf16 [n, >= Hq*hd]."""
+    nb, hkv, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    if (hkv, d) != (Hkv, hd) or Hq <= 0 or Hq % Hkv or Hq // Hkv > 16:
+        raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
+    _check_rows("q", q, (0,), Hq * hd)
+    _check_rows("out", out, (0,), Hq * hd)
+    n = q.shape[0]
+    if out.shape[0] != n or (n > 1 and out.stride(0) < Hq * hd):
+        raise ValueError(f"out must have {n} rows that do not overlap")
+    _check_index("ctx_len", ctx_len, n)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1 \
+            or not block_table.is_contiguous():
+        raise ValueError(f"block_table must be contiguous int32 [{n}, width]")
+    dev = _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
+    need = _decode_bytes(n, Hq, Hkv, hd, dev.index) if n else 0
+    if ws.numel() * ws.element_size() < need or not ws.is_contiguous():
+        raise ValueError(f"workspace of {ws.numel() * ws.element_size()} bytes, {need} needed in a row")
+    _launch(dev, "artb_paged_decode_q8", _lib.ptr(q), q.stride(0), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale),
+            _lib.ptr(v_scale), _lib.ptr(block_table), block_table.shape[1], _lib.ptr(ctx_len), bs, n, Hq, Hkv, hd, _lib.ptr(out),
+            out.stride(0), _lib.ptr(ws), nb, KINDS[k_cache.dtype])
+    return out
