@@ -199,81 +199,66 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
       }
       return x;
     };
-    // the blocks of a tile's two stretches, -1: no keys there
+    // the blocks of a tile's two stretches; the second may have no keys, and is then read where the first lies
     auto blocks_of = [&](const PqAt& x, bool any, int (&blk)[2]) {
+      const int* row = block_table + static_cast<size_t>(x.seq) * max_blocks;
+      const int last = (x.len - 1) >> 4;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int sb = x.tile * 2 + s;
-        blk[s] = any && sb * 16 < x.len
-                     ? __ldcg(block_table + static_cast<size_t>(x.seq) * max_blocks + (sub_shift >= 0 ? sb >> sub_shift : sb / subs))
-                     : -1;
+        const int sb = min(x.tile * 2 + s, last);
+        blk[s] = any ? __ldcg(row + (sub_shift >= 0 ? sb >> sub_shift : sb / subs)) : 0;
       }
     };
-    auto check_blocks = [&](const PqAt& x, int (&blk)[2]) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if ((blk[s] < 0 || blk[s] >= num_blocks) && (x.tile * 2 + s) * 16 < x.len) {
-          if (status) atomicMax(status, ST_BOUNDS);
-          blk[s] = -2;                       // keys whose block is none: left out
-        }
-    };
-    auto place = [&](const PqAt& x, int s) { return ((x.tile * 2 + s) - (sub_shift >= 0 ? ((x.tile * 2 + s) >> sub_shift) << sub_shift : (x.tile * 2 + s) / subs * subs)) * 16; };
-
     uint32_t kr[2][2][KW], vr[2][4][VW];
     float ks[2], vs[2], ks_next[2], vs_next[2];
-    auto load_k = [&](const PqAt& x, const int (&blk)[2], float (&scale)[2]) {
+    int keys[2], keys_next[2];                      // of each stretch: 16, fewer at a context's end, 0 where its block is none
+    size_t off[2];                                  // of the stretch that is being requested, in the codes of keys and of values
+    uint32_t head[2];                               // and its scale
+    const uint8_t* k_lane = k_cache + g * HD + t * (HD / 4);
+    const uint8_t* v_lane = v_cache + 2 * t * HD + g * (HD / 8);
+    auto load_k = [&](const PqAt& x, const int (&blk)[2], int (&n)[2], float (&scale)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        scale[s] = 0.f;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int i = 0; i < KW; ++i) kr[s][r][i] = 0;
-        if (blk[s] >= 0) {
-          const size_t head = static_cast<size_t>(blk[s]) * Hkv + kvh;
-          const uint8_t* p = k_cache + (head * block_size + place(x, s) + g) * HD + t * (HD / 4);
-          pq_load<HD / 4>(kr[s][0], p);
-          pq_load<HD / 4>(kr[s][1], p + 8 * HD);
-          scale[s] = __ldcg(k_scale + head);
-        }
+        const int sb = min(x.tile * 2 + s, (x.len - 1) >> 4);
+        const bool good = static_cast<unsigned>(blk[s]) < static_cast<unsigned long>(num_blocks);
+        if (!good && status) atomicMax(status, ST_BOUNDS);
+        n[s] = good ? max(0, min(16, x.len - (x.tile * 2 + s) * 16)) : 0;
+        head[s] = static_cast<uint32_t>(good ? blk[s] : 0) * Hkv + kvh;
+        off[s] = static_cast<size_t>(head[s]) * (block_size * HD) + (sb - (sub_shift >= 0 ? sb >> sub_shift << sub_shift : sb / subs * subs)) * (16 * HD);
+        pq_load<HD / 4>(kr[s][0], k_lane + off[s]);
+        pq_load<HD / 4>(kr[s][1], k_lane + off[s] + 8 * HD);
+        scale[s] = __ldcg(k_scale + head[s]);
       }
     };
-    auto load_v = [&](const PqAt& x, const int (&blk)[2], float (&scale)[2]) {
+    auto load_v = [&](float (&scale)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        scale[s] = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int i = 0; i < VW; ++i) vr[s][r][i] = 0;
-        if (blk[s] >= 0) {
-          const size_t head = static_cast<size_t>(blk[s]) * Hkv + kvh;
-          const uint8_t* p = v_cache + (head * block_size + place(x, s) + 2 * t) * HD + g * (HD / 8);
-          const int left = x.len - (x.tile * 2 + s) * 16 - 2 * t;       // what lies behind the context may be any bits
-          if (left > 0) pq_load<HD / 8>(vr[s][0], p);
-          if (left > 1) pq_load<HD / 8>(vr[s][1], p + HD);
-          if (left > 8) pq_load<HD / 8>(vr[s][2], p + 8 * HD);
-          if (left > 9) pq_load<HD / 8>(vr[s][3], p + 9 * HD);
-          scale[s] = __ldcg(v_scale + head);
-        }
+        pq_load<HD / 8>(vr[s][0], v_lane + off[s]);
+        pq_load<HD / 8>(vr[s][1], v_lane + off[s] + HD);
+        pq_load<HD / 8>(vr[s][2], v_lane + off[s] + 8 * HD);
+        pq_load<HD / 8>(vr[s][3], v_lane + off[s] + 9 * HD);
+        scale[s] = __ldcg(v_scale + head[s]);
       }
     };
 
     PqAt a = s_start[warp];
-    int blk[2], blk_next[2], first = s_first[warp], piece_lo = a.tile;
-    blocks_of(a, true, blk);
+    int blk_next[2], first = s_first[warp], piece_lo = a.tile;
+    {
+      int blk[2];
+      blocks_of(a, true, blk);
+      load_k(a, blk, keys, ks);
+      load_v(vs);
+    }
     PqAt b = next(a);
     blocks_of(b, count_tiles > 1, blk_next);
-    check_blocks(a, blk);
-    load_k(a, blk, ks);
-    load_v(a, blk, vs);
 
     uint32_t qf[NT][JT][2];
-    float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4];
+    float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4], unit, per_unit;
     bool fresh = true;
     for (int i = 0; i < count_tiles; ++i) {
       if (fresh) {
         fresh = false;
+        unit = per_unit = 0.f;
         // heads g (and g + 8), hd / 4 values from t * hd / 4 on: the order in which the lanes hold the keys
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -335,31 +320,42 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
           for (int n = 0; n < NT; ++n) pq_mma(s[u][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
         }
       }
-      if (i + 1 < count_tiles) {
-        check_blocks(b, blk_next);
-        load_k(b, blk_next, ks_next);
+      if (i + 1 < count_tiles) load_k(b, blk_next, keys_next, ks_next);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float f0 = qs[n][0] * ks[u], f1 = qs[n][1] * ks[u];
+          s[u][n][0] *= f0;
+          s[u][n][1] *= f1;
+          s[u][n][2] *= f0;
+          s[u][n][3] *= f1;
+        }
+      if (keys[0] + keys[1] < PQ_KEYS) {            // a context's last tile; what lies behind it may be any bits
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (g + (x >> 1) * 8 >= keys[u]) s[u][n][x] = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+              if (2 * t + (r & 1) + (r >> 1) * 8 >= keys[u]) vr[u][r][w] = 0;
+          if (keys[u] == 0) vs[u] = 0.f;
+        }
       }
       bool moves = false;
       float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) top[n][x] = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int left = blk[u] >= 0 ? a.len - (a.tile * 2 + u) * 16 - g : 0;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[u][n][x] = left > (x >> 1) * 8 ? s[u][n][x] * (qs[n][x & 1] * ks[u]) : -INFINITY;
-            top[n][x & 1] = fmaxf(top[n][x & 1], s[u][n][x]);
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) moves |= top[n][x] > m[n][x] + PQ_SLACK;
+        for (int x = 0; x < 2; ++x) {
+          top[n][x] = fmaxf(fmaxf(s[0][n][x], s[0][n][2 + x]), fmaxf(s[1][n][x], s[1][n][2 + x]));
+          moves |= top[n][x] > m[n][x] + PQ_SLACK;
+        }
       // weights are relative to a reference that need not be the maximum: while no score passes it by more than 2^8, which
       // fp16 and the sums bear, it stays, and with it everything summed so far
       if (__any_sync(0xffffffffu, moves)) {
@@ -380,23 +376,29 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
             }
           }
       }
-      uint32_t pf[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float r0 = m[n][0] == -INFINITY ? 0.f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float p0 = pq_exp2(s[u][n][0] - r0), p1 = pq_exp2(s[u][n][1] - r1);
-          const float p2 = pq_exp2(s[u][n][2] - r0), p3 = pq_exp2(s[u][n][3] - r1);
-          l[n][0] += p0 + p2;
-          l[n][1] += p1 + p3;
-          pf[u][n][0] = pq_transpose(pq_half2(p0, p1));
-          pf[u][n][1] = pq_transpose(pq_half2(p2, p3));
+          s[u][n][0] = pq_exp2(s[u][n][0] - r0);
+          s[u][n][1] = pq_exp2(s[u][n][1] - r1);
+          s[u][n][2] = pq_exp2(s[u][n][2] - r0);
+          s[u][n][3] = pq_exp2(s[u][n][3] - r1);
+          l[n][0] += s[u][n][0] + s[u][n][2];
+          l[n][1] += s[u][n][1] + s[u][n][3];
         }
       }
-      // values: rows are hd / 8 neighbouring values per g, two to a product
+      // Adds a stretch's values.  Sums are held in units of a scale: a weight is multiplied by the ratio of its own block's scale
+      // to the unit before it is rounded.  Rows of the product are hd / 8 neighbouring values per g, two to a product.
+      auto add = [&](int u) {
+        const float ratio = vs[u] * per_unit;
+        uint32_t pf[NT][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int n = 0; n < NT; ++n) {
+          pf[n][0] = pq_transpose(pq_half2(s[u][n][0] * ratio, s[u][n][1] * ratio));
+          pf[n][1] = pq_transpose(pq_half2(s[u][n][2] * ratio, s[u][n][3] * ratio));
+        }
 #pragma unroll
         for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -406,14 +408,33 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
             pq_widen<KIND>(__byte_perm(vr[u][0][w], vr[u][1][w], sel), a0, a1);
             pq_widen<KIND>(__byte_perm(vr[u][2][w], vr[u][3][w], sel), a2, a3);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              pq_mma(d, a0, a1, a2, a3, pf[u][n][0], pf[u][n][1]);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) acc[n][2 * w + half][x] = fmaf(vs[u], d[x], acc[n][2 * w + half][x]);
-            }
+            for (int n = 0; n < NT; ++n) pq_mma(acc[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
           }
-      if (i + 1 < count_tiles) load_v(b, blk_next, vs_next);
+      };
+      // The unit follows the scales when a ratio leaves [1/2, 64], so that weights keep their fp16 precision and range whatever
+      // the scales of a sequence's blocks are.
+      auto fits = [&](float x) { return (x >= 0.5f * unit && x <= 64.f * unit) || x == 0.f; };
+      if (fits(vs[0]) && fits(vs[1])) {
+        add(0);
+        add(1);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (!fits(vs[u])) {
+            const float f = fminf(unit / vs[u], 1.2e27f);    // 2^90: beside sums that large a weight is nothing
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[n][j][x] *= f;
+            unit = unit == 0.f ? vs[u] : unit / f;
+            per_unit = 1.f / unit;
+          }
+          add(u);
+        }
+      }
+      if (i + 1 < count_tiles) load_v(vs_next);
 
       const int tiles = tiles_in(a.len);
       if (i + 1 == count_tiles || a.tile + 1 == tiles) {
@@ -428,6 +449,11 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const int head = n * 8 + 2 * t + x;
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+              acc[n][j][x] *= unit;
+              acc[n][j][2 + x] *= unit;
+            }
             if (whole) {
               if (head < G) {
                 __nv_bfloat16* o_row = out + static_cast<size_t>(a.seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
@@ -455,7 +481,7 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
       b = c;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        blk[u] = blk_next[u];
+        keys[u] = keys_next[u];
         blk_next[u] = blk_after[u];
         ks[u] = ks_next[u];
         vs[u] = vs_next[u];
@@ -591,7 +617,7 @@ ARTB_EXPORT int artb_paged_decode_q8(const void* q, int ldq, const void* k_cache
                                      int block_size, int num_seqs, int Hq, int Hkv, int hd, void* out, int ldo, void* ws,
                                      long num_blocks, int kind, int* status, cudaStream_t st) {
   if (num_seqs <= 0) return 0;
-  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || block_size < 16 || (block_size & 15) || max_blocks < 1 || (ldq & 7) ||
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || block_size < 16 || (block_size & 15) || max_blocks < 1 || num_blocks < 1 || (ldq & 7) ||
       (ldo & 7) || !ws)
     return ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
