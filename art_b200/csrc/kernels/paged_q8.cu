@@ -4,13 +4,11 @@
 // The G = Hq / Hkv query heads of a kv head are the columns of one m16n8 tile (two for G > 8), so that keys and values are
 // read once for all of them.  Both products have the cache's side as their rows,
 //     S^T [16 keys x heads] = K Q^T,     O^T [hd x heads] = V^T P^T,
-// and 16 keys are always of one block: a scale is one factor of a score tile and of a value tile's product, and no code is
-// ever multiplied by it.  Codes become fp16 (exact: e4m3 and int8 have at most 8 significant bits), queries too, after a power
-// of two per head that brings their largest to 2^14 (exact but for what is 2^-38 of it); weights are rounded to fp16.
-//
-// No shared memory on the way in.  The order in which a product sums is free, so each lane loads the bytes that its own
-// fragments need, in 16-byte pieces: hd / 4 neighbouring values of its keys, and hd / 8 neighbouring values of four keys, whose
-// bytes are paired up in registers while they are widened.
+// and 16 keys are always of one block: a key scale is one factor of a tile of scores, a value scale one of a tile of weights, and
+// no code is ever multiplied by either.  Codes become fp16 (exact: e4m3 and int8 have at most 8 significant bits), queries too,
+// after a power of two per head that brings their largest to 2^14 (exact but for what is 2^-38 of it); weights are rounded to
+// fp16.  The order in which a product sums is free, so a lane's fragments are neighbouring bytes: hd / 4 values of a key, and
+// hd / 8 values of four keys, whose bytes are paired up in registers while they are widened.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -22,28 +20,49 @@
 namespace artb {
 
 constexpr int PQ_KEYS = 32;              // keys of a tile: two stretches of 16, each within a block
-constexpr int PQ_MIN_TILES = 4;          // tiles of a CTA at least: one per warp
-constexpr int PQ_LENS = 256;             // context lengths that a CTA keeps at hand
+constexpr int PQ_WARPS = 4;              // that compute; one more brings the tiles
+constexpr int PQ_THREADS = (PQ_WARPS + 1) * 32;
+constexpr int PQ_MIN_TILES = PQ_WARPS;   // tiles of a CTA at least: one per warp
+constexpr int PQ_LENS = 1024;            // context lengths that a CTA keeps at hand
+constexpr int PQ_ROUND = 32 / PQ_WARPS;  // tiles of each warp that are looked up at a time
+constexpr int PQ_NOTES = 2 * PQ_ROUND;   // what is noted about a warp's tiles: this round's and the one in use
 constexpr float PQ_SLACK = 8.f;          // how far (in powers of two) a score may pass the reference before that moves
 
 __host__ __device__ constexpr int pq_heads(int G) { return G > 8 ? 16 : 8; }
-// by registers: a warp holds 8 * PQ_KEYS / 32 * hd bytes of keys and values and hd * heads sums
-__host__ __device__ constexpr int pq_ctas_per_sm(int hd, int heads) { return hd == 128 ? (heads == 8 ? 3 : 2) : hd == 64 && heads == 16 ? 3 : 4; }
+__host__ __device__ constexpr int pq_stages(int hd) { return hd == 128 ? 2 : hd == 64 ? 3 : 4; }       // tiles of a warp in shared memory
+__host__ __device__ constexpr int pq_ctas_per_sm(int hd) { return hd == 128 ? 2 : 3; }  // by shared memory
 __host__ __device__ constexpr int pq_piece_floats(int heads, int hd) { return heads * hd + ((2 * heads + 3) & ~3); }
 
+template <int HD, int HEADS>
+struct PqSmem {
+  static constexpr int STRETCH = 16 * HD, STAGE = 4 * STRETCH, RING = pq_stages(HD) * STAGE;      // keys, keys, values, values
+  static constexpr int PIECE = pq_piece_floats(HEADS, HD) * 4;
+  static constexpr int BYTES = 1024 + PQ_WARPS * (RING + PIECE);                                    // rings begin on 1024 bytes
+  static_assert(PIECE <= RING, "a warp's last piece goes where its tiles were");
+};
+
 template <int BYTES>
-__device__ __forceinline__ void pq_load(uint32_t* r, const uint8_t* p) {
+__device__ __forceinline__ void pq_take(uint32_t* r, const uint8_t* p) {
   if (BYTES == 4) {
-    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
   } else if (BYTES == 8) {
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x;
+    r[1] = v.y;
   } else {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i)
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(r[4 * i]), "=r"(r[4 * i + 1]), "=r"(r[4 * i + 2]), "=r"(r[4 * i + 3])
-                   : "l"(p + 16 * i));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[0] = v.x;
+    r[1] = v.y;
+    r[2] = v.z;
+    r[3] = v.w;
   }
+}
+
+// Where 16-byte piece `piece` of row `row` of a stretch lies: the copies spread a row's pieces by the row's number, so that the
+// lanes of a fragment find theirs in different banks.
+template <int HD>
+__device__ __forceinline__ int pq_piece_at(int row, int piece) {
+  return row * HD + ((piece ^ (HD == 128 ? row & 7 : HD == 64 ? row >> 1 & 3 : row >> 2 & 1)) << 4);
 }
 
 // Four codes to two pairs of fp16: bytes 0, 1 and bytes 2, 3.
@@ -93,9 +112,15 @@ __device__ __forceinline__ void pq_store4(__nv_bfloat16* dst, const float4& o, f
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Where a warp stands in the tiles of all sequences.
-struct PqAt {
-  int seq, tile, len;
+// The first tile of a warp: tile `tile` of a sequence whose first tile is number `first` of all.
+struct PqStart {
+  int seq, len, first;
+};
+
+// What a computing warp has to know of a tile beside its codes.
+struct __align__(16) PqNote {
+  int tile, len, keys[2];      // tile of the sequence, keys of each stretch: 16, fewer at a context's end, 0 where its block is none
+  float ks[2], vs[2];
 };
 
 // What a warp leaves of a sequence that it has not read whole: tiles [lo, hi) of the sequence whose first tile is `first`.
@@ -105,29 +130,45 @@ struct PqPiece {
 
 // The sequences are laid end to end, in tiles of PQ_KEYS keys, and cut into equal shares, wherever sequences begin and end in
 // them; a share belongs to Hkv neighbouring CTAs, one per kv head, and the shares together fill the chip once.  A CTA's share is
-// cut again into four, one per warp.  A warp goes through its tiles without a stop at the ends of sequences: keys of the next
-// tile are requested as soon as the scores have been taken from those of this one, values once they have been added up, and
-// table entries a tile before that.  A sequence that one warp reads whole is written by it.  The pieces of others meet in shared
-// memory, and what still is a part then goes to the workspace; the CTA that finishes last adds the parts up in their order.
+// cut again into four, one per computing warp, which goes through its tiles without a stop at the ends of sequences.  The
+// fifth warp brings the tiles: its lanes look up the next eight of each warp (sequence, blocks, scales) while those before are
+// on their way, and a tile's copies start as soon as its warp has left the stage.  A sequence that one warp reads whole is
+// written by it.  The pieces of others meet in shared memory, and what still is a part then goes to the workspace; the CTA that
+// finishes last adds the parts up in their order.
 template <int KIND, int HD, int HEADS>
-__global__ void __launch_bounds__(128, pq_ctas_per_sm(HD, HEADS))
-paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8_t* __restrict__ k_cache,
-                       const uint8_t* __restrict__ v_cache, const float* __restrict__ k_scale, const float* __restrict__ v_scale,
-                       const int* __restrict__ block_table, int max_blocks, const int* __restrict__ ctx_len, int block_size,
-                       int nseq, int Hq, int Hkv, __nv_bfloat16* __restrict__ out, int ldo, float* part, int* count,
-                       float scale_log2, long num_blocks, int* status) {
-  constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32;
-  constexpr int PF = pq_piece_floats(HEADS, HD);
-  extern __shared__ __align__(16) float pq_smem[];          // [8 pieces][PF]: sums [HEADS][HD], reference [HEADS], sum [HEADS]
-  __shared__ int s_warp[4], s_len[PQ_LENS], s_done;
-  __shared__ PqAt s_start[4];
-  __shared__ int s_first[4];
-  __shared__ PqPiece s_piece[8];
-  pdl_wait();
+__global__ void __launch_bounds__(PQ_THREADS, pq_ctas_per_sm(HD))
+paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const __nv_bfloat16* __restrict__ q, int ldq, const float* __restrict__ k_scale,
+                       const float* __restrict__ v_scale, const int* __restrict__ block_table, int max_blocks,
+                       const int* __restrict__ ctx_len, int block_size, int nseq, int Hq, int Hkv,
+                       __nv_bfloat16* __restrict__ out, int ldo, float* part, int* count, float scale_log2, long num_blocks,
+                       int* status) {
+  using S = PqSmem<HD, HEADS>;
+  constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD);
+  extern __shared__ uint8_t pq_smem_raw[];
+  uint8_t* rings = pq_smem_raw + (1024 - (smem_u32(pq_smem_raw) & 1023));
+  __shared__ int s_warp[PQ_WARPS], s_len[PQ_LENS], s_done;
+  __shared__ volatile int s_abort;
+  __shared__ PqStart s_start[PQ_WARPS];
+  __shared__ PqPiece s_piece[2 * PQ_WARPS];
+  __shared__ PqNote s_note[PQ_WARPS][PQ_NOTES];
+  __shared__ __align__(8) uint64_t s_full[PQ_WARPS][STAGES], s_empty[PQ_WARPS][STAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid < PQ_WARPS * STAGES) {
+    mbar_init(&s_full[0][0] + tid, 1);
+    mbar_init(&s_empty[0][0] + tid, 1);
+    fence_mbar_init();
+  }
+  if (tid < 2 * PQ_WARPS) s_piece[tid].seq = -1;
+  if (tid == PQ_THREADS - 1) {
+    s_abort = 0;
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  pdl_wait();
   const int G = Hq / Hkv, shares = gridDim.x / Hkv, share = blockIdx.x / Hkv, kvh = blockIdx.x - share * Hkv;
   const int table_keys = min(static_cast<long>(max_blocks) * block_size, 0x7fffffffL - PQ_KEYS);
-  auto length = [&](int i) {
+  auto read_len = [&](int i) {
     int n = ctx_len[i];
     if (n > table_keys) {
       if (blockIdx.x == 0 && status) atomicMax(status, ST_BOUNDS);
@@ -135,13 +176,15 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
     }
     return max(n, 0);
   };
+  auto length = [&](int i) { return nseq <= PQ_LENS ? s_len[i] : read_len(i); };
   auto tiles_in = [](int len) { return (len + PQ_KEYS - 1) / PQ_KEYS; };
 
   // where the share begins: each thread sums the tiles of a run of sequences, then a scan over the threads
   const int run = (nseq + 127) / 128, i0 = min(nseq, tid * run), i1 = min(nseq, i0 + run);
   int own = 0;
   for (int i = i0; i < i1; ++i) {
-    const int len = length(i);
+    const int len = read_len(i);
+    if (nseq <= PQ_LENS) s_len[i] = len;
     own += tiles_in(len);
     if (len == 0 && share == shares - 1) {           // an empty context (the padding of a batch): zeros
       uint4* o = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * ldo + kvh * G * HD);
@@ -154,20 +197,19 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_warp[warp] = incl;
-  if (tid < 8) s_piece[tid].seq = -1;
+  if (lane == 31 && warp < PQ_WARPS) s_warp[warp] = incl;
   __syncthreads();
   int total = 0, before = incl - own;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < PQ_WARPS; ++w) {
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
-  const int per = max(PQ_MIN_TILES, (total + shares - 1) / shares), per_warp = (per + 3) / 4;
+  const int per = max(PQ_MIN_TILES, (total + shares - 1) / shares), per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
   const int at = share * per;
   if (at >= total) return;                  // the whole CTA
   const int end = min(total, at + per);
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < PQ_WARPS; ++w) {
     const int x = at + w * per_warp;
     if (x < end && before <= x && x < before + own) {
       int i = i0, b = before, len;
@@ -177,94 +219,108 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
         if (x < b + n) break;
         b += n;
       }
-      s_start[w] = PqAt{i, x - b, len};
-      s_first[w] = b;
+      s_start[w] = PqStart{i, len, b};
     }
   }
   __syncthreads();
-  const int seq0 = s_start[0].seq;
-  for (int i = tid; i < PQ_LENS; i += 128) s_len[i] = seq0 + i < nseq ? length(seq0 + i) : 0x7fffffff - PQ_KEYS;
-  __syncthreads();
 
-  const int lo = at + warp * per_warp, count_tiles = min(end, lo + per_warp) - lo;
-  if (count_tiles > 0) {
-    const int subs = block_size / 16, sub_shift = (subs & (subs - 1)) == 0 ? 31 - __clz(subs) : -1;
-    auto next = [&](PqAt x) {
-      if (++x.tile * PQ_KEYS >= x.len) {
-        x.tile = 0;
-        do {
-          ++x.seq;
-          x.len = x.seq - seq0 < PQ_LENS ? s_len[x.seq - seq0] : x.seq < nseq ? length(x.seq) : 0x7fffffff - PQ_KEYS;
-        } while (x.len <= 0);
-      }
-      return x;
+  if (warp == PQ_WARPS) {
+    // ------------------------------------------------------------------ bringing tiles
+    const int w = lane % PQ_WARPS, turn = lane / PQ_WARPS, lo = at + w * per_warp, tiles = max(0, min(end, lo + per_warp) - lo);
+    const int most = min(end - at, per_warp), subs = block_size / 16;
+    PqStart cur = tiles > 0 ? s_start[w] : PqStart{0, 0, 0};
+    struct Tile {
+      int seq, tile, len, blk[2], keys[2], row[2];
+      float ks[2], vs[2];
     };
-    // the blocks of a tile's two stretches; the second may have no keys, and is then read where the first lies
-    auto blocks_of = [&](const PqAt& x, bool any, int (&blk)[2]) {
-      const int* row = block_table + static_cast<size_t>(x.seq) * max_blocks;
-      const int last = (x.len - 1) >> 4;
+    // this lane's tile of a round: which it is, and its blocks on their way
+    auto find = [&](int i, Tile& x) {
+      if (i >= tiles) return;
+      while (lo + i >= cur.first + tiles_in(cur.len)) {
+        cur.first += tiles_in(cur.len);
+        cur.len = length(++cur.seq);
+      }
+      x.seq = cur.seq;
+      x.len = cur.len;
+      x.tile = lo + i - cur.first;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int sb = min(x.tile * 2 + s, last);
-        blk[s] = any ? __ldcg(row + (sub_shift >= 0 ? sb >> sub_shift : sb / subs)) : 0;
+      for (int u = 0; u < 2; ++u) {
+        x.keys[u] = max(0, min(16, x.len - (x.tile * 2 + u) * 16));
+        x.blk[u] = x.keys[u] > 0 ? __ldcg(block_table + static_cast<size_t>(x.seq) * max_blocks + (x.tile * 2 + u) / subs) : 0;
       }
     };
-    uint32_t kr[2][2][KW], vr[2][4][VW];
-    float ks[2], vs[2], ks_next[2], vs_next[2];
-    int keys[2], keys_next[2];                      // of each stretch: 16, fewer at a context's end, 0 where its block is none
-    size_t off[2];                                  // of the stretch that is being requested, in the codes of keys and of values
-    uint32_t head[2];                               // and its scale
-    const uint8_t* k_lane = k_cache + g * HD + t * (HD / 4);
-    const uint8_t* v_lane = v_cache + 2 * t * HD + g * (HD / 8);
-    auto load_k = [&](const PqAt& x, const int (&blk)[2], int (&n)[2], float (&scale)[2]) {
+    // its rows in the codes, and its scales on their way
+    auto place = [&](int i, Tile& x) {
+      if (i >= tiles) return;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int sb = min(x.tile * 2 + s, (x.len - 1) >> 4);
-        const bool good = static_cast<unsigned>(blk[s]) < static_cast<unsigned long>(num_blocks);
-        if (!good && status) atomicMax(status, ST_BOUNDS);
-        n[s] = good ? max(0, min(16, x.len - (x.tile * 2 + s) * 16)) : 0;
-        head[s] = static_cast<uint32_t>(good ? blk[s] : 0) * Hkv + kvh;
-        off[s] = static_cast<size_t>(head[s]) * (block_size * HD) + (sb - (sub_shift >= 0 ? sb >> sub_shift << sub_shift : sb / subs * subs)) * (16 * HD);
-        pq_load<HD / 4>(kr[s][0], k_lane + off[s]);
-        pq_load<HD / 4>(kr[s][1], k_lane + off[s] + 8 * HD);
-        scale[s] = __ldcg(k_scale + head[s]);
+      for (int u = 0; u < 2; ++u) {
+        x.ks[u] = x.vs[u] = 0.f;
+        if (x.keys[u] > 0 && !q8_index_ok(x.blk[u], num_blocks, status)) x.keys[u] = 0;
+        if (x.keys[u] > 0) {
+          const long head = static_cast<long>(x.blk[u]) * Hkv + kvh;
+          x.row[u] = static_cast<int>(head * block_size + (x.tile * 2 + u) % subs * 16);
+          x.ks[u] = __ldcg(k_scale + head);
+          x.vs[u] = __ldcg(v_scale + head);
+        }
       }
     };
-    auto load_v = [&](float (&scale)[2]) {
+    Tile now, later;
+    find(turn, now);
+    place(turn, now);
+    for (int base = 0; base < most; base += PQ_ROUND) {
+      if (__any_sync(0xffffffffu, s_abort)) break;
+      find(base + PQ_ROUND + turn, later);
+      for (int r = 0; r < PQ_ROUND; ++r) {
+        const int i = base + r, stage = i % STAGES;
+        if (turn == r && i < tiles && !s_abort) {
+          if (!mbar_wait_timed(&s_empty[w][stage], (i / STAGES & 1) ^ 1)) {
+            if (status) atomicMax(status, ST_TIMEOUT_EMPTY);
+            s_abort = 1;
+          } else {
+            uint8_t* to = rings + w * S::RING + stage * S::STAGE;
+            int bytes = 0;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        pq_load<HD / 8>(vr[s][0], v_lane + off[s]);
-        pq_load<HD / 8>(vr[s][1], v_lane + off[s] + HD);
-        pq_load<HD / 8>(vr[s][2], v_lane + off[s] + 8 * HD);
-        pq_load<HD / 8>(vr[s][3], v_lane + off[s] + 9 * HD);
-        scale[s] = __ldcg(v_scale + head[s]);
+            for (int u = 0; u < 2; ++u)
+              if (now.keys[u] > 0) {
+                tma_load_2d(to + u * S::STRETCH, &k_map, 0, now.row[u], &s_full[w][stage]);
+                tma_load_2d(to + (2 + u) * S::STRETCH, &v_map, 0, now.row[u], &s_full[w][stage]);
+                bytes += 2 * S::STRETCH;
+              }
+            PqNote* n = &s_note[w][i % PQ_NOTES];
+            *reinterpret_cast<int4*>(n) = make_int4(now.tile, now.len, now.keys[0], now.keys[1]);
+            *reinterpret_cast<float4*>(n->ks) = make_float4(now.ks[0], now.ks[1], now.vs[0], now.vs[1]);
+            mbar_expect_tx(&s_full[w][stage], bytes);       // after the copies: these need not wait for the scales
+          }
+        }
+        __syncwarp();
+        if (r == PQ_ROUND / 2) place(base + PQ_ROUND + turn, later);
       }
-    };
-
-    PqAt a = s_start[warp];
-    int blk_next[2], first = s_first[warp], piece_lo = a.tile;
-    {
-      int blk[2];
-      blocks_of(a, true, blk);
-      load_k(a, blk, keys, ks);
-      load_v(vs);
+      now = later;
     }
-    PqAt b = next(a);
-    blocks_of(b, count_tiles > 1, blk_next);
+  } else if (at + warp * per_warp < end) {
+    // ------------------------------------------------------------------ computing
+    const int lo = at + warp * per_warp, tiles = min(end, lo + per_warp) - lo;
+    uint8_t* ring = rings + warp * S::RING;
+    int seq = s_start[warp].seq, first = s_start[warp].first, piece_lo = lo - first;
+    // this lane's bytes of a stretch: of the keys g and g + 8, and of the values 2t, 2t + 1 (and 8 further)
+    const int k_at[2] = {HD == 32 ? pq_piece_at<HD>(g, t >> 1) + (t & 1) * 8 : pq_piece_at<HD>(g, HD == 128 ? 2 * t : t),
+                         HD == 128 ? pq_piece_at<HD>(g, 2 * t + 1) : 0};
+    const int v_piece = HD == 128 ? g : HD == 64 ? g >> 1 : g >> 2, v_rest = HD == 128 ? 0 : HD == 64 ? (g & 1) * 8 : (g & 3) * 4;
+    const int v_at[2] = {pq_piece_at<HD>(2 * t, v_piece) + v_rest, pq_piece_at<HD>(2 * t + 1, v_piece) + v_rest};
 
     uint32_t qf[NT][JT][2];
     float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4], unit, per_unit;
     bool fresh = true;
-    for (int i = 0; i < count_tiles; ++i) {
+    for (int i = 0; i < tiles; ++i) {
       if (fresh) {
         fresh = false;
         unit = per_unit = 0.f;
-        // heads g (and g + 8), hd / 4 values from t * hd / 4 on: the order in which the lanes hold the keys
+        // heads g (and g + 8), hd / 4 values: those that the lane holds of a key, in the same order
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           uint32_t raw[JT * 2], top = 0;
           const int head = n * 8 + g;
-          const __nv_bfloat16* row = q + static_cast<size_t>(a.seq) * ldq + (kvh * G + head) * HD + t * (HD / 4);
+          const __nv_bfloat16* row = q + static_cast<size_t>(seq) * ldq + (kvh * G + head) * HD + t * (HD / 4);
 #pragma unroll
           for (int v = 0; v < JT * 2 / 4; ++v) {
             const uint4 x = head < G ? __ldcg(reinterpret_cast<const uint4*>(row) + v) : make_uint4(0, 0, 0, 0);
@@ -299,14 +355,35 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
             for (int x = 0; x < 4; ++x) acc[n][j][x] = 0.f;
         }
       }
-      const PqAt c = next(b);
-      int blk_after[2];
-      blocks_of(c, i + 2 < count_tiles, blk_after);
+      const int stage = i % STAGES;
+      const uint8_t* codes = ring + stage * S::STAGE;
+      const bool came = mbar_wait_timed(&s_full[warp][stage], i / STAGES & 1);
+      if (!__all_sync(0xffffffffu, came)) {
+        if (status) atomicMax(status, ST_TIMEOUT_FULL);
+        s_abort = 1;
+        break;
+      }
+      const int4 n0 = *reinterpret_cast<const int4*>(&s_note[warp][i % PQ_NOTES]);
+      const float4 n1 = *reinterpret_cast<const float4*>(s_note[warp][i % PQ_NOTES].ks);
+      const int tile = n0.x, len = n0.y, keys[2] = {n0.z, n0.w};
+      const float ks[2] = {n1.x, n1.y};
+      float vs[2] = {n1.z, n1.w};
 
       // scores: rows are the keys g and g + 8 of a stretch, columns the heads 2t and 2t + 1
       float s[2][NT][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        uint32_t kr[2][KW];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* p = codes + u * S::STRETCH + r * 8 * HD;
+          if (HD == 32) {
+            pq_take<8>(kr[r], p + k_at[0]);
+          } else {
+            pq_take<16>(kr[r], p + k_at[0]);
+            if (HD == 128) pq_take<16>(kr[r] + KW / 2, p + k_at[1]);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -314,13 +391,19 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
           uint32_t a0, a1, a2, a3;
-          pq_widen<KIND>(kr[u][0][j], a0, a2);
-          pq_widen<KIND>(kr[u][1][j], a1, a3);
+          pq_widen<KIND>(kr[0][j], a0, a2);
+          pq_widen<KIND>(kr[1][j], a1, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) pq_mma(s[u][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
         }
       }
-      if (i + 1 < count_tiles) load_k(b, blk_next, keys_next, ks_next);
+      uint32_t vr[2][4][VW];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pq_take<VW * 4>(vr[u][r], codes + (2 + u) * S::STRETCH + (r >> 1) * 8 * HD + v_at[r & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[warp][stage]);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -434,13 +517,12 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
           add(u);
         }
       }
-      if (i + 1 < count_tiles) load_v(vs_next);
 
-      const int tiles = tiles_in(a.len);
-      if (i + 1 == count_tiles || a.tile + 1 == tiles) {
-        const bool whole = piece_lo == 0 && a.tile + 1 == tiles;
-        const int where = warp * 2 + (piece_lo == 0);
-        float* piece = pq_smem + where * PF;
+      if (i + 1 == tiles || tile + 1 == tiles_in(len)) {
+        const bool whole = piece_lo == 0 && tile + 1 == tiles_in(len);
+        // the last piece goes where the tiles were
+        float* piece = reinterpret_cast<float*>(i + 1 == tiles ? ring : rings + PQ_WARPS * S::RING + warp * S::PIECE);
+        __syncwarp();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -456,7 +538,7 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
             }
             if (whole) {
               if (head < G) {
-                __nv_bfloat16* o_row = out + static_cast<size_t>(a.seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
+                __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
 #pragma unroll
                 for (int j = 0; j < JT; j += 2)
                   pq_store4(o_row + 2 * j, make_float4(acc[n][j][x], acc[n][j][2 + x], acc[n][j + 1][x], acc[n][j + 1][2 + x]), sum);
@@ -472,34 +554,33 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
               }
             }
           }
-        if (!whole && lane == 0) s_piece[where] = PqPiece{a.seq, a.len, first, piece_lo, a.tile + 1};
+        if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, first, piece_lo, tile + 1};
         first = lo + i + 1;                   // the next sequence begins with the next tile
         piece_lo = 0;
         fresh = true;
-      }
-      a = b;
-      b = c;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        keys[u] = keys_next[u];
-        blk_next[u] = blk_after[u];
-        ks[u] = ks_next[u];
-        vs[u] = vs_next[u];
+        if (i + 1 < tiles) do ++seq; while (length(seq) == 0);
       }
     }
   }
   pdl_launch_dependents();
   __syncthreads();
+  if (s_abort) {                              // no copy may outlive the CTA
+    if (warp < PQ_WARPS && lane < STAGES) mbar_wait_timed(&s_full[warp][lane], 0, 100), mbar_wait_timed(&s_full[warp][lane], 1, 100);
+    return;
+  }
 
   // the pieces in their order: neighbours of one sequence are added up
-  for (int p0 = 0; p0 < 8;) {
+  auto piece_of = [&](int p) {
+    return reinterpret_cast<const float*>(p & 1 ? rings + (p >> 1) * S::RING : rings + PQ_WARPS * S::RING + (p >> 1) * S::PIECE);
+  };
+  for (int p0 = 0; p0 < 2 * PQ_WARPS;) {
     const PqPiece head_piece = s_piece[p0];
     if (head_piece.seq < 0) {
       ++p0;
       continue;
     }
     int p1 = p0 + 1, hi = head_piece.hi;
-    for (int p = p0 + 1; p < 8; ++p) {
+    for (int p = p0 + 1; p < 2 * PQ_WARPS; ++p) {
       if (s_piece[p].seq < 0) continue;
       if (s_piece[p].seq != head_piece.seq) break;
       hi = s_piece[p].hi;
@@ -512,15 +593,15 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
     const int slot_floats = pq_piece_floats(G, HD);
     auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
     float* w = slot(share, head_piece.lo == 0);
-    for (int idx = tid; idx < G * (HD / 4); idx += 128) {
+    for (int idx = tid; idx < G * (HD / 4); idx += PQ_THREADS) {
       const int r = idx / (HD / 4);
       float mm = -INFINITY, sum = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int p = p0; p < p1; ++p)
-        if (s_piece[p].seq >= 0) mm = fmaxf(mm, pq_smem[p * PF + HEADS * HD + r]);
+        if (s_piece[p].seq >= 0) mm = fmaxf(mm, piece_of(p)[HEADS * HD + r]);
       for (int p = p0; p < p1; ++p) {
         if (s_piece[p].seq < 0) continue;
-        const float* x = pq_smem + p * PF;
+        const float* x = piece_of(p);
         const float mp = x[HEADS * HD + r], f = mp == -INFINITY ? (x[HEADS * HD + HEADS + r] == 0.f ? 0.f : 1.f) : pq_exp2(mp - mm);
         const float4 v = *reinterpret_cast<const float4*>(x + idx * 4);
         sum = fmaf(x[HEADS * HD + HEADS + r], f, sum);
@@ -544,7 +625,7 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
       __syncthreads();
       if (s_done) {
         __threadfence();
-        for (int idx = tid; idx < G * HD / 4; idx += 128) {
+        for (int idx = tid; idx < G * HD / 4; idx += PQ_THREADS) {
           const int r = idx / (HD / 4);
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
           float mx = -INFINITY, sum = 0.f;
@@ -584,19 +665,26 @@ paged_decode_q8_kernel(const __nv_bfloat16* __restrict__ q, int ldq, const uint8
   }
 }
 
-template <int HD, int HEADS>
-constexpr int pq_smem_bytes() {
-  return 8 * pq_piece_floats(HEADS, HD) * 4;
-}
-
 // whole shares: one CTA per kv head in each
-static int pq_grid(int hd, int Hq, int Hkv) {
-  const int shares = sm_count() * pq_ctas_per_sm(hd, pq_heads(Hq / Hkv)) / Hkv;
+static int pq_grid(int hd, int Hkv) {
+  const int shares = sm_count() * pq_ctas_per_sm(hd) / Hkv;
   return (shares < 1 ? 1 : shares) * Hkv;
 }
 
 static long pq_part_bytes(int Hq, int Hkv, int hd) {
-  return (static_cast<long>(pq_grid(hd, Hq, Hkv)) * 2 * pq_piece_floats(Hq / Hkv, hd) * 4 + 15) / 16 * 16;
+  return (static_cast<long>(pq_grid(hd, Hkv)) * 2 * pq_piece_floats(Hq / Hkv, hd) * 4 + 15) / 16 * 16;
+}
+
+// The codes as rows of hd bytes, brought 16 at a time.
+static int pq_map(CUtensorMap* map, const void* codes, long rows, int hd) {
+  auto enc = get_tmap_encoder();
+  if (!enc) return ERR_NO_DRIVER;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(hd)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(hd), 16}, steps[2] = {1, 1};
+  const CUtensorMapSwizzle spread = hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : hd == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, spread, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : ERR_TMAP;
 }
 
 }  // namespace artb
@@ -623,26 +711,31 @@ ARTB_EXPORT int artb_paged_decode_q8(const void* q, int ldq, const void* k_cache
   if ((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
        reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
     return ERR_BAD_ALIGN;
+  if (num_blocks * Hkv * block_size > 0x7fffffffL) return ERR_TOO_LARGE;        // rows are numbered with 31 bits
   int dev_ = 0;
   if (cudaGetDevice(&dev_) != cudaSuccess || dev_ < 0 || dev_ >= 64) return ERR_BAD_SHAPE;
   const float scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
   float* part = static_cast<float*>(ws);
   int* count = reinterpret_cast<int*>(static_cast<char*>(ws) + pq_part_bytes(Hq, Hkv, hd));
   const int heads = pq_heads(Hq / Hkv);
+  if (hd != 128 && hd != 64 && hd != 32) return ERR_BAD_SHAPE;
+  CUtensorMap k_map, v_map;
+  int rc = pq_map(&k_map, k_cache, num_blocks * Hkv * block_size, hd);
+  if (!rc) rc = pq_map(&v_map, v_cache, num_blocks * Hkv * block_size, hd);
+  if (rc) return rc;
 #define ARTB_PQ(KIND_, HD_, HEADS_)                                                                                           \
   if (kind == KIND_ && hd == HD_ && heads == HEADS_) {                                                                        \
     static bool cfgd[64] = {false};   /* the attribute is per device */                                                       \
     if (!cfgd[dev_]) {                                                                                                        \
       cudaError_t e = cudaFuncSetAttribute(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                           pq_smem_bytes<HD_, HEADS_>());                                                     \
+                                           PqSmem<HD_, HEADS_>::BYTES);                                                       \
       if (e != cudaSuccess) return static_cast<int>(e);                                                                       \
       cfgd[dev_] = true;                                                                                                      \
     }                                                                                                                         \
-    return static_cast<int>(launch_kernel(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(pq_grid(HD_, Hq, Hkv)), dim3(128), \
-                                          pq_smem_bytes<HD_, HEADS_>(), st, (const __nv_bfloat16*)q, ldq,                     \
-                                          (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, block_table,    \
-                                          max_blocks, ctx_len, block_size, num_seqs, Hq, Hkv, (__nv_bfloat16*)out, ldo, part, \
-                                          count, scale_log2, num_blocks, status));                                            \
+    return static_cast<int>(launch_kernel(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(pq_grid(HD_, Hkv)), dim3(PQ_THREADS), \
+                                          PqSmem<HD_, HEADS_>::BYTES, st, k_map, v_map, (const __nv_bfloat16*)q, ldq,         \
+                                          k_scale, v_scale, block_table, max_blocks, ctx_len, block_size, num_seqs, Hq, Hkv,  \
+                                          (__nv_bfloat16*)out, ldo, part, count, scale_log2, num_blocks, status));            \
   }
 #define ARTB_PQ_KIND(KIND_)                                                                                                   \
   ARTB_PQ(KIND_, 128, 8) ARTB_PQ(KIND_, 128, 16) ARTB_PQ(KIND_, 64, 8) ARTB_PQ(KIND_, 64, 16) ARTB_PQ(KIND_, 32, 8)           \
