@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(PQ_THREADS, pq_ctas_per_sm(HD))
 paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                        const __nv_bfloat16* __restrict__ q, int ldq, const float* __restrict__ k_scale,
                        const float* __restrict__ v_scale, const int* __restrict__ block_table, int max_blocks,
-                       const int* __restrict__ ctx_len, int block_size, int nseq, int Hq, int Hkv,
-                       __nv_bfloat16* __restrict__ out, int ldo, float* part, int* count, float scale_log2, long num_blocks,
-                       int* status) {
+                       const int* __restrict__ ctx_len, int block_size, int sub_shift, int nseq, int G,
+                       uint32_t per_share, __nv_bfloat16* __restrict__ out, int ldo, float* part, int* count, float scale_log2,
+                       long num_blocks, int* status) {
   using S = PqSmem<HD, HEADS>;
   constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD);
   extern __shared__ uint8_t pq_smem_raw[];
@@ -166,12 +166,12 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     tma_prefetch_desc(&v_map);
   }
   pdl_wait();
-  const int G = Hq / Hkv, shares = gridDim.x / Hkv, share = blockIdx.x / Hkv, kvh = blockIdx.x - share * Hkv;
+  const int Hkv = gridDim.x, kvh = blockIdx.x, shares = gridDim.y, share = blockIdx.y;
   const int table_keys = min(static_cast<long>(max_blocks) * block_size, 0x7fffffffL - PQ_KEYS);
   auto read_len = [&](int i) {
     int n = ctx_len[i];
     if (n > table_keys) {
-      if (blockIdx.x == 0 && status) atomicMax(status, ST_BOUNDS);
+      if (kvh == 0 && share == 0 && status) atomicMax(status, ST_BOUNDS);
       n = table_keys;
     }
     return max(n, 0);
@@ -205,10 +205,11 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
-  const int per = max(PQ_MIN_TILES, (total + shares - 1) / shares), per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
+  const int per = max(PQ_MIN_TILES, static_cast<int>(__umulhi(total + shares - 1, per_share)) + (shares == 1)), per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
   const int at = share * per;
   if (at >= total) return;                  // the whole CTA
   const int end = min(total, at + per);
+#pragma unroll 1
   for (int w = 0; w < PQ_WARPS; ++w) {
     const int x = at + w * per_warp;
     if (x < end && before <= x && x < before + own) {
@@ -227,7 +228,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   if (warp == PQ_WARPS) {
     // ------------------------------------------------------------------ bringing tiles
     const int w = lane % PQ_WARPS, turn = lane / PQ_WARPS, lo = at + w * per_warp, tiles = max(0, min(end, lo + per_warp) - lo);
-    const int most = min(end - at, per_warp), subs = block_size / 16;
+    const int most = min(end - at, per_warp), subs = block_size >> 4;
+    auto block_of = [&](int stretch) { return sub_shift >= 0 ? stretch >> sub_shift : stretch / subs; };
     PqStart cur = tiles > 0 ? s_start[w] : PqStart{0, 0, 0};
     struct Tile {
       int seq, tile, len, blk[2], keys[2], row[2];
@@ -246,7 +248,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         x.keys[u] = max(0, min(16, x.len - (x.tile * 2 + u) * 16));
-        x.blk[u] = x.keys[u] > 0 ? __ldcg(block_table + static_cast<size_t>(x.seq) * max_blocks + (x.tile * 2 + u) / subs) : 0;
+        x.blk[u] = x.keys[u] > 0 ? __ldcg(block_table + static_cast<size_t>(x.seq) * max_blocks + block_of(x.tile * 2 + u)) : 0;
       }
     };
     // its rows in the codes, and its scales on their way
@@ -258,7 +260,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (x.keys[u] > 0 && !q8_index_ok(x.blk[u], num_blocks, status)) x.keys[u] = 0;
         if (x.keys[u] > 0) {
           const long head = static_cast<long>(x.blk[u]) * Hkv + kvh;
-          x.row[u] = static_cast<int>(head * block_size + (x.tile * 2 + u) % subs * 16);
+          x.row[u] = static_cast<int>(head * block_size + (x.tile * 2 + u - block_of(x.tile * 2 + u) * subs) * 16);
           x.ks[u] = __ldcg(k_scale + head);
           x.vs[u] = __ldcg(v_scale + head);
         }
@@ -496,26 +498,24 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       };
       // The unit follows the scales when a ratio leaves [1/2, 64], so that weights keep their fp16 precision and range whatever
       // the scales of a sequence's blocks are.
-      auto fits = [&](float x) { return (x >= 0.5f * unit && x <= 64.f * unit) || x == 0.f; };
-      if (fits(vs[0]) && fits(vs[1])) {
-        add(0);
-        add(1);
-      } else {
+      if (unit == 0.f) {
+        unit = vs[0] != 0.f ? vs[0] : vs[1];
+        per_unit = unit != 0.f ? rcp_approx(unit) : 0.f;
+      }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (!fits(vs[u])) {
-            const float f = fminf(unit / vs[u], 1.2e27f);    // 2^90: beside sums that large a weight is nothing
+      for (int u = 0; u < 2; ++u) {
+        if (!(vs[u] >= 0.5f * unit && vs[u] <= 64.f * unit) && vs[u] != 0.f) {
+          const float f = fminf(unit * rcp_approx(vs[u]), 0x1p90f);        // beside sums that large a weight is nothing
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < JT; ++j)
+            for (int j = 0; j < JT; ++j)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[n][j][x] *= f;
-            unit = unit == 0.f ? vs[u] : unit / f;
-            per_unit = 1.f / unit;
-          }
-          add(u);
+              for (int x = 0; x < 4; ++x) acc[n][j][x] *= f;
+          unit = f < 0x1p90f ? vs[u] : unit * 0x1p-90f;
+          per_unit = rcp_approx(unit);
         }
+        add(u);
       }
 
       if (i + 1 == tiles || tile + 1 == tiles_in(len)) {
@@ -569,90 +569,107 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     return;
   }
 
-  // the pieces in their order: neighbours of one sequence are added up
+  // The pieces in their order: neighbours of one sequence, at most one per warp, are added up.
   auto piece_of = [&](int p) {
     return reinterpret_cast<const float*>(p & 1 ? rings + (p >> 1) * S::RING : rings + PQ_WARPS * S::RING + (p >> 1) * S::PIECE);
   };
-  for (int p0 = 0; p0 < 2 * PQ_WARPS;) {
-    const PqPiece head_piece = s_piece[p0];
-    if (head_piece.seq < 0) {
-      ++p0;
-      continue;
+  const int slot_floats = pq_piece_floats(G, HD), items = G * (HD / 4);
+  // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
+  auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
+  // what holds nothing has no reference, or has met a value that is not a number
+  auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : pq_exp2(m - top); };
+  const int my_seq = lane < 2 * PQ_WARPS ? s_piece[lane].seq : -1;
+  uint32_t todo = __ballot_sync(0xffffffffu, my_seq >= 0);
+  while (todo) {
+    const int p0 = __ffs(todo) - 1, seq = __shfl_sync(0xffffffffu, my_seq, p0);
+    const uint32_t mine = __ballot_sync(0xffffffffu, my_seq == seq);
+    todo &= ~mine;
+    const PqPiece front = s_piece[p0];
+    const int hi = s_piece[31 - __clz(mine)].hi, tiles = tiles_in(front.len);
+    const bool whole = front.lo == 0 && hi == tiles;
+    const float* from[PQ_WARPS];
+    uint32_t rest = mine;
+#pragma unroll
+    for (int w = 0; w < PQ_WARPS; ++w) {
+      from[w] = rest ? piece_of(__ffs(rest) - 1) : nullptr;
+      rest &= rest - 1;
     }
-    int p1 = p0 + 1, hi = head_piece.hi;
-    for (int p = p0 + 1; p < 2 * PQ_WARPS; ++p) {
-      if (s_piece[p].seq < 0) continue;
-      if (s_piece[p].seq != head_piece.seq) break;
-      hi = s_piece[p].hi;
-      p1 = p + 1;
-    }
-    const int seq = head_piece.seq, first = head_piece.first, tiles = tiles_in(head_piece.len);
-    const bool whole = head_piece.lo == 0 && hi == tiles;
     __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + kvh * G * HD;
-    // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
-    const int slot_floats = pq_piece_floats(G, HD);
-    auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
-    float* w = slot(share, head_piece.lo == 0);
-    for (int idx = tid; idx < G * (HD / 4); idx += PQ_THREADS) {
+    float* to = slot(share, front.lo == 0);
+#pragma unroll 2
+    for (int idx = tid; idx < items; idx += PQ_THREADS) {
       const int r = idx / (HD / 4);
-      float mm = -INFINITY, sum = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p = p0; p < p1; ++p)
-        if (s_piece[p].seq >= 0) mm = fmaxf(mm, piece_of(p)[HEADS * HD + r]);
-      for (int p = p0; p < p1; ++p) {
-        if (s_piece[p].seq < 0) continue;
-        const float* x = piece_of(p);
-        const float mp = x[HEADS * HD + r], f = mp == -INFINITY ? (x[HEADS * HD + HEADS + r] == 0.f ? 0.f : 1.f) : pq_exp2(mp - mm);
-        const float4 v = *reinterpret_cast<const float4*>(x + idx * 4);
-        sum = fmaf(x[HEADS * HD + HEADS + r], f, sum);
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+      float m[PQ_WARPS], l[PQ_WARPS], top = -INFINITY, sum = 0.f;
+      float4 v[PQ_WARPS], o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < PQ_WARPS; ++w) {
+        m[w] = -INFINITY;
+        l[w] = 0.f;
+        v[w] = o;
+        if (from[w]) {
+          m[w] = from[w][HEADS * HD + r];
+          l[w] = from[w][HEADS * HD + HEADS + r];
+          v[w] = *reinterpret_cast<const float4*>(from[w] + idx * 4);
+        }
+        top = fmaxf(top, m[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < PQ_WARPS; ++w) {
+        const float f = weight(m[w], l[w], top);
+        sum = fmaf(l[w], f, sum);
+        o = make_float4(fmaf(v[w].x, f, o.x), fmaf(v[w].y, f, o.y), fmaf(v[w].z, f, o.z), fmaf(v[w].w, f, o.w));
       }
       if (whole) {
         pq_store4(o_row + idx * 4, o, sum);
       } else {
-        *reinterpret_cast<float4*>(w + idx * 4) = o;
+        __stcg(reinterpret_cast<float4*>(to + idx * 4), o);
         if (idx * 4 == r * HD) {
-          w[G * HD + r] = mm;
-          w[G * HD + G + r] = sum;
+          __stcg(to + G * HD + r, top);
+          __stcg(to + G * HD + G + r, sum);
         }
       }
     }
     if (!whole) {
-      __threadfence();
       __syncthreads();
-      const int sh0 = first / per, parts = (first + tiles - 1) / per - sh0 + 1;
-      if (tid == 0) s_done = atomicAdd(&count[seq * Hkv + kvh], 1) == parts - 1;
+      const int sh0 = front.first / per, parts = (front.first + tiles - 1) / per - sh0 + 1;
+      if (tid == 0) {
+        __threadfence();                                     // of what the CTA wrote before the barrier
+        s_done = atomicAdd(&count[seq * Hkv + kvh], 1) == parts - 1;
+        __threadfence();
+      }
       __syncthreads();
       if (s_done) {
-        __threadfence();
-        for (int idx = tid; idx < G * HD / 4; idx += PQ_THREADS) {
+#pragma unroll 2
+        for (int idx = tid; idx < items; idx += PQ_THREADS) {
           const int r = idx / (HD / 4);
+          float top = -INFINITY, sum = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float mx = -INFINITY, sum = 0.f;
-          for (int q0 = 0; q0 < parts; q0 += 8) {          // eight parts' loads in flight
-            float m[8], l[8];
+          for (int q0 = 0; q0 < parts; q0 += 8) {            // eight parts' loads in flight
+            float m[8], l[8], now = top;
             float4 v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float* sl = slot(sh0 + min(q0 + j, parts - 1), q0 + j == 0);
-              m[j] = __ldcg(sl + G * HD + r);
-              l[j] = __ldcg(sl + G * HD + G + r);
-              v[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx);
+              m[j] = -INFINITY;
+              l[j] = 0.f;
+              v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (q0 + j < parts) {
+                const float* sl = slot(sh0 + q0 + j, q0 + j == 0);
+                m[j] = __ldcg(sl + G * HD + r);
+                l[j] = __ldcg(sl + G * HD + G + r);
+                v[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx);
+              }
             }
-            float mn = mx;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mn = fmaxf(mn, q0 + j < parts ? m[j] : -INFINITY);
-            const float c = mx == -INFINITY ? 1.f : pq_exp2(mx - mn);        // nothing yet, or what has no reference
-            mx = mn;
-            o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+            for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
+            const float c = top == -INFINITY ? 1.f : pq_exp2(top - now);
+            top = now;
             sum *= c;
+            o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float f = q0 + j >= parts ? 0.f : m[j] == -INFINITY ? (l[j] == 0.f ? 0.f : 1.f) : pq_exp2(m[j] - mn);
-              if (f != 0.f) {
-                sum = fmaf(l[j], f, sum);
-                o = make_float4(fmaf(v[j].x, f, o.x), fmaf(v[j].y, f, o.y), fmaf(v[j].z, f, o.z), fmaf(v[j].w, f, o.w));
-              }
+              const float f = weight(m[j], l[j], now);
+              sum = fmaf(l[j], f, sum);
+              o = make_float4(fmaf(v[j].x, f, o.x), fmaf(v[j].y, f, o.y), fmaf(v[j].z, f, o.z), fmaf(v[j].w, f, o.w));
             }
           }
           pq_store4(o_row + idx * 4, o, sum);
@@ -661,18 +678,17 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       __syncthreads();                                       // s_done is read before the next part sets it
     }
-    p0 = p1;
   }
 }
 
 // whole shares: one CTA per kv head in each
-static int pq_grid(int hd, int Hkv) {
+static int pq_shares(int hd, int Hkv) {
   const int shares = sm_count() * pq_ctas_per_sm(hd) / Hkv;
-  return (shares < 1 ? 1 : shares) * Hkv;
+  return shares < 1 ? 1 : shares;
 }
 
 static long pq_part_bytes(int Hq, int Hkv, int hd) {
-  return (static_cast<long>(pq_grid(hd, Hkv)) * 2 * pq_piece_floats(Hq / Hkv, hd) * 4 + 15) / 16 * 16;
+  return (static_cast<long>(pq_shares(hd, Hkv)) * Hkv * 2 * pq_piece_floats(Hq / Hkv, hd) * 4 + 15) / 16 * 16;
 }
 
 // The codes as rows of hd bytes, brought 16 at a time.
@@ -719,6 +735,9 @@ ARTB_EXPORT int artb_paged_decode_q8(const void* q, int ldq, const void* k_cache
   int* count = reinterpret_cast<int*>(static_cast<char*>(ws) + pq_part_bytes(Hq, Hkv, hd));
   const int heads = pq_heads(Hq / Hkv);
   if (hd != 128 && hd != 64 && hd != 32) return ERR_BAD_SHAPE;
+  const int shares = pq_shares(hd, Hkv), subs = block_size / 16, sub_shift = (subs & (subs - 1)) ? -1 : __builtin_ctz(subs);
+  // 2^32 / shares, rounded up: a share is a product instead of a division, and never too small
+  const uint32_t per_share = shares == 1 ? 0xffffffffu : static_cast<uint32_t>(((1ull << 32) + shares - 1) / shares);
   CUtensorMap k_map, v_map;
   int rc = pq_map(&k_map, k_cache, num_blocks * Hkv * block_size, hd);
   if (!rc) rc = pq_map(&v_map, v_cache, num_blocks * Hkv * block_size, hd);
@@ -732,10 +751,11 @@ ARTB_EXPORT int artb_paged_decode_q8(const void* q, int ldq, const void* k_cache
       if (e != cudaSuccess) return static_cast<int>(e);                                                                       \
       cfgd[dev_] = true;                                                                                                      \
     }                                                                                                                         \
-    return static_cast<int>(launch_kernel(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(pq_grid(HD_, Hkv)), dim3(PQ_THREADS), \
+    return static_cast<int>(launch_kernel(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(Hkv, shares), dim3(PQ_THREADS),       \
                                           PqSmem<HD_, HEADS_>::BYTES, st, k_map, v_map, (const __nv_bfloat16*)q, ldq,         \
-                                          k_scale, v_scale, block_table, max_blocks, ctx_len, block_size, num_seqs, Hq, Hkv,  \
-                                          (__nv_bfloat16*)out, ldo, part, count, scale_log2, num_blocks, status));            \
+                                          k_scale, v_scale, block_table, max_blocks, ctx_len, block_size, sub_shift, num_seqs, \
+                                          Hq / Hkv, per_share, (__nv_bfloat16*)out, ldo, part, count, scale_log2, num_blocks, \
+                                          status));                                                                           \
   }
 #define ARTB_PQ_KIND(KIND_)                                                                                                   \
   ARTB_PQ(KIND_, 128, 8) ARTB_PQ(KIND_, 128, 16) ARTB_PQ(KIND_, 64, 8) ARTB_PQ(KIND_, 64, 16) ARTB_PQ(KIND_, 32, 8)           \
