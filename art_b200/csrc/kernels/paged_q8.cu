@@ -20,22 +20,23 @@
 namespace artb {
 
 constexpr int PQ_KEYS = 32;              // keys of a tile: two stretches of 16, each within a block
-constexpr int PQ_WARPS = 4;              // that compute; one more brings the tiles
-constexpr int PQ_THREADS = (PQ_WARPS + 1) * 32;
+constexpr int PQ_WARPS = 4;
+constexpr int PQ_THREADS = PQ_WARPS * 32;
 constexpr int PQ_MIN_TILES = PQ_WARPS;   // tiles of a CTA at least: one per warp
-constexpr int PQ_LENS = 1024;            // context lengths that a CTA keeps at hand
-constexpr int PQ_ROUND = 32 / PQ_WARPS;  // tiles of each warp that are looked up at a time
-constexpr int PQ_NOTES = 2 * PQ_ROUND;   // what is noted about a warp's tiles: this round's and the one in use
+constexpr int PQ_ENTRIES = 1024;         // of a CTA's list of where sequences begin
+constexpr int PQ_ROUND = 16;             // tiles that a warp looks up at a time
+constexpr int PQ_NOTES = 2 * PQ_ROUND;   // and keeps noted: those in use and the next
 constexpr float PQ_SLACK = 8.f;          // how far (in powers of two) a score may pass the reference before that moves
 
 __host__ __device__ constexpr int pq_heads(int G) { return G > 8 ? 16 : 8; }
-__host__ __device__ constexpr int pq_stages(int hd) { return hd == 128 ? 2 : hd == 64 ? 3 : 4; }       // tiles of a warp in shared memory
+// tiles of a warp in shared memory
+__host__ __device__ constexpr int pq_stages(int hd, int heads) { return hd == 128 ? 2 : hd == 64 ? (heads == 8 ? 3 : 2) : 4; }
 __host__ __device__ constexpr int pq_ctas_per_sm(int hd) { return hd == 128 ? 2 : 3; }  // by shared memory
 __host__ __device__ constexpr int pq_piece_floats(int heads, int hd) { return heads * hd + ((2 * heads + 3) & ~3); }
 
 template <int HD, int HEADS>
 struct PqSmem {
-  static constexpr int STRETCH = 16 * HD, STAGE = 4 * STRETCH, RING = pq_stages(HD) * STAGE;      // keys, keys, values, values
+  static constexpr int STRETCH = 16 * HD, STAGE = 4 * STRETCH, RING = pq_stages(HD, HEADS) * STAGE;      // keys, keys, values, values
   static constexpr int PIECE = pq_piece_floats(HEADS, HD) * 4;
   static constexpr int BYTES = 1024 + PQ_WARPS * (RING + PIECE);                                    // rings begin on 1024 bytes
   static_assert(PIECE <= RING, "a warp's last piece goes where its tiles were");
@@ -106,21 +107,36 @@ __device__ __forceinline__ uint32_t pq_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void pq_store4(__nv_bfloat16* dst, const float4& o, float sum) {
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const __nv_bfloat162 a = __floats2bfloat162_rn(o.x * inv, o.y * inv), b = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ void pq_store4(__nv_bfloat16* dst, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
 }
-
-// The first tile of a warp: tile `tile` of a sequence whose first tile is number `first` of all.
-struct PqStart {
-  int seq, len, first;
+// A weighted sum of pieces: eight values of a head, and the sum of its weights.
+struct PqSum {
+  float4 a, b;
+  float l;
+  __device__ __forceinline__ void add(const float4& x, const float4& y, float sum, float f) {
+    a = make_float4(fmaf(x.x, f, a.x), fmaf(x.y, f, a.y), fmaf(x.z, f, a.z), fmaf(x.w, f, a.w));
+    b = make_float4(fmaf(y.x, f, b.x), fmaf(y.y, f, b.y), fmaf(y.z, f, b.z), fmaf(y.w, f, b.w));
+    l = fmaf(sum, f, l);
+  }
+  __device__ __forceinline__ void scale(float f) {
+    a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+    b = make_float4(b.x * f, b.y * f, b.z * f, b.w * f);
+    l *= f;
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* dst) const {
+    const float inv = l == 0.f ? 0.f : rcp_approx(l);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv),
+                                                pack_bf16x2(b.x * inv, b.y * inv), pack_bf16x2(b.z * inv, b.w * inv));
+  }
 };
 
-// What a computing warp has to know of a tile beside its codes.
+// A tile: which of its sequence's it is; keys of each stretch (16, fewer at a context's end, 0 where its block is none), their rows
+// in the codes and their scales.
 struct __align__(16) PqNote {
-  int tile, len, keys[2];      // tile of the sequence, keys of each stretch: 16, fewer at a context's end, 0 where its block is none
+  int seq, tile, len, keys;                 // keys: first stretch | second << 8
   float ks[2], vs[2];
+  int row[2], none[2];
 };
 
 // What a warp leaves of a sequence that it has not read whole: tiles [lo, hi) of the sequence whose first tile is `first`.
@@ -130,9 +146,9 @@ struct PqPiece {
 
 // The sequences are laid end to end, in tiles of PQ_KEYS keys, and cut into equal shares, wherever sequences begin and end in
 // them; a share belongs to Hkv neighbouring CTAs, one per kv head, and the shares together fill the chip once.  A CTA's share is
-// cut again into four, one per computing warp, which goes through its tiles without a stop at the ends of sequences.  The
-// fifth warp brings the tiles: its lanes look up the next eight of each warp (sequence, blocks, scales) while those before are
-// on their way, and a tile's copies start as soon as its warp has left the stage.  A sequence that one warp reads whole is
+// cut again into four, one per warp, which goes through its tiles without a stop at the ends of sequences: its lanes look up
+// sixteen tiles at a time (sequence, blocks, then scales) while those before are in use, and a tile's copies into shared memory
+// start as soon as the warp has taken the last bytes of the one whose place it gets.  A sequence that one warp reads whole is
 // written by it.  The pieces of others meet in shared memory, and what still is a part then goes to the workspace; the CTA that
 // finishes last adds the parts up in their order.
 template <int KIND, int HD, int HEADS>
@@ -144,19 +160,17 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                        uint32_t per_share, __nv_bfloat16* __restrict__ out, int ldo, float* part, int* count, float scale_log2,
                        long num_blocks, int* status) {
   using S = PqSmem<HD, HEADS>;
-  constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD);
+  constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD, HEADS);
   extern __shared__ uint8_t pq_smem_raw[];
   uint8_t* rings = pq_smem_raw + (1024 - (smem_u32(pq_smem_raw) & 1023));
-  __shared__ int s_warp[PQ_WARPS], s_len[PQ_LENS], s_done;
+  __shared__ int s_warp[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES], s_done;
   __shared__ volatile int s_abort;
-  __shared__ PqStart s_start[PQ_WARPS];
   __shared__ PqPiece s_piece[2 * PQ_WARPS];
   __shared__ PqNote s_note[PQ_WARPS][PQ_NOTES];
-  __shared__ __align__(8) uint64_t s_full[PQ_WARPS][STAGES], s_empty[PQ_WARPS][STAGES];
+  __shared__ __align__(8) uint64_t s_full[PQ_WARPS][STAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (tid < PQ_WARPS * STAGES) {
     mbar_init(&s_full[0][0] + tid, 1);
-    mbar_init(&s_empty[0][0] + tid, 1);
     fence_mbar_init();
   }
   if (tid < 2 * PQ_WARPS) s_piece[tid].seq = -1;
@@ -176,19 +190,26 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     }
     return max(n, 0);
   };
-  auto length = [&](int i) { return nseq <= PQ_LENS ? s_len[i] : read_len(i); };
   auto tiles_in = [](int len) { return (len + PQ_KEYS - 1) / PQ_KEYS; };
 
-  // where the share begins: each thread sums the tiles of a run of sequences, then a scan over the threads
-  const int run = (nseq + 127) / 128, i0 = min(nseq, tid * run), i1 = min(nseq, i0 + run);
+  // Where sequences begin, in tiles: an entry for each (for `run` of them where there are very many), each thread's entries
+  // first for themselves, then a scan over the threads.
+  const int run = (nseq + PQ_ENTRIES - 1) / PQ_ENTRIES, entries = (nseq + run - 1) / run, mine = (entries + PQ_THREADS - 1) / PQ_THREADS;
+  const int e0 = min(entries, tid * mine), e1 = min(entries, e0 + mine);
   int own = 0;
-  for (int i = i0; i < i1; ++i) {
-    const int len = read_len(i);
-    if (nseq <= PQ_LENS) s_len[i] = len;
-    own += tiles_in(len);
-    if (len == 0 && share == shares - 1) {           // an empty context (the padding of a batch): zeros
-      uint4* o = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * ldo + kvh * G * HD);
-      for (int d = 0; d < G * HD / 8; ++d) o[d] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int e = e0; e < e1; ++e) {
+    s_first[e] = own;
+#pragma unroll 1
+    for (int i = e * run; i < min(nseq, (e + 1) * run); ++i) {
+      const int len = read_len(i);
+      s_len[e] = len;                                  // used where run is 1
+      own += tiles_in(len);
+      if (len == 0 && share == shares - 1) {           // an empty context (the padding of a batch): zeros
+        uint4* o = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * ldo + kvh * G * HD);
+#pragma unroll 1
+        for (int d = 0; d < G * HD / 8; ++d) o[d] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
   int incl = own;
@@ -197,7 +218,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31 && warp < PQ_WARPS) s_warp[warp] = incl;
+  if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
   int total = 0, before = incl - own;
 #pragma unroll
@@ -205,105 +226,91 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
   }
+#pragma unroll 1
+  for (int e = e0; e < e1; ++e) s_first[e] += before;
   const int per = max(PQ_MIN_TILES, static_cast<int>(__umulhi(total + shares - 1, per_share)) + (shares == 1)), per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
   const int at = share * per;
   if (at >= total) return;                  // the whole CTA
   const int end = min(total, at + per);
-#pragma unroll 1
-  for (int w = 0; w < PQ_WARPS; ++w) {
-    const int x = at + w * per_warp;
-    if (x < end && before <= x && x < before + own) {
-      int i = i0, b = before, len;
-      for (;; ++i) {
-        len = length(i);
-        const int n = tiles_in(len);
-        if (x < b + n) break;
-        b += n;
-      }
-      s_start[w] = PqStart{i, len, b};
-    }
-  }
   __syncthreads();
 
-  if (warp == PQ_WARPS) {
-    // ------------------------------------------------------------------ bringing tiles
-    const int w = lane % PQ_WARPS, turn = lane / PQ_WARPS, lo = at + w * per_warp, tiles = max(0, min(end, lo + per_warp) - lo);
-    const int most = min(end - at, per_warp), subs = block_size >> 4;
-    auto block_of = [&](int stretch) { return sub_shift >= 0 ? stretch >> sub_shift : stretch / subs; };
-    PqStart cur = tiles > 0 ? s_start[w] : PqStart{0, 0, 0};
-    struct Tile {
-      int seq, tile, len, blk[2], keys[2], row[2];
-      float ks[2], vs[2];
-    };
-    // this lane's tile of a round: which it is, and its blocks on their way
-    auto find = [&](int i, Tile& x) {
-      if (i >= tiles) return;
-      while (lo + i >= cur.first + tiles_in(cur.len)) {
-        cur.first += tiles_in(cur.len);
-        cur.len = length(++cur.seq);
-      }
-      x.seq = cur.seq;
-      x.len = cur.len;
-      x.tile = lo + i - cur.first;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        x.keys[u] = max(0, min(16, x.len - (x.tile * 2 + u) * 16));
-        x.blk[u] = x.keys[u] > 0 ? __ldcg(block_table + static_cast<size_t>(x.seq) * max_blocks + block_of(x.tile * 2 + u)) : 0;
-      }
-    };
-    // its rows in the codes, and its scales on their way
-    auto place = [&](int i, Tile& x) {
-      if (i >= tiles) return;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        x.ks[u] = x.vs[u] = 0.f;
-        if (x.keys[u] > 0 && !q8_index_ok(x.blk[u], num_blocks, status)) x.keys[u] = 0;
-        if (x.keys[u] > 0) {
-          const long head = static_cast<long>(x.blk[u]) * Hkv + kvh;
-          x.row[u] = static_cast<int>(head * block_size + (x.tile * 2 + u - block_of(x.tile * 2 + u) * subs) * 16);
-          x.ks[u] = __ldcg(k_scale + head);
-          x.vs[u] = __ldcg(v_scale + head);
-        }
-      }
-    };
-    Tile now, later;
-    find(turn, now);
-    place(turn, now);
-    for (int base = 0; base < most; base += PQ_ROUND) {
-      if (__any_sync(0xffffffffu, s_abort)) break;
-      find(base + PQ_ROUND + turn, later);
-      for (int r = 0; r < PQ_ROUND; ++r) {
-        const int i = base + r, stage = i % STAGES;
-        if (turn == r && i < tiles && !s_abort) {
-          if (!mbar_wait_timed(&s_empty[w][stage], (i / STAGES & 1) ^ 1)) {
-            if (status) atomicMax(status, ST_TIMEOUT_EMPTY);
-            s_abort = 1;
-          } else {
-            uint8_t* to = rings + w * S::RING + stage * S::STAGE;
-            int bytes = 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (now.keys[u] > 0) {
-                tma_load_2d(to + u * S::STRETCH, &k_map, 0, now.row[u], &s_full[w][stage]);
-                tma_load_2d(to + (2 + u) * S::STRETCH, &v_map, 0, now.row[u], &s_full[w][stage]);
-                bytes += 2 * S::STRETCH;
-              }
-            PqNote* n = &s_note[w][i % PQ_NOTES];
-            *reinterpret_cast<int4*>(n) = make_int4(now.tile, now.len, now.keys[0], now.keys[1]);
-            *reinterpret_cast<float4*>(n->ks) = make_float4(now.ks[0], now.ks[1], now.vs[0], now.vs[1]);
-            mbar_expect_tx(&s_full[w][stage], bytes);       // after the copies: these need not wait for the scales
-          }
-        }
-        __syncwarp();
-        if (r == PQ_ROUND / 2) place(base + PQ_ROUND + turn, later);
-      }
-      now = later;
-    }
-  } else if (at + warp * per_warp < end) {
-    // ------------------------------------------------------------------ computing
-    const int lo = at + warp * per_warp, tiles = min(end, lo + per_warp) - lo;
+  const int lo = at + warp * per_warp, tiles = min(end, lo + per_warp) - lo;
+  if (tiles > 0) {
     uint8_t* ring = rings + warp * S::RING;
-    int seq = s_start[warp].seq, first = s_start[warp].first, piece_lo = lo - first;
+    PqNote* notes = s_note[warp];
+    const int subs = block_size >> 4;
+    PqNote next;                            // this lane's tile of the round that is being looked up
+    int blk[2];
+    auto find = [&](int i) {                // which it is, and its blocks on their way
+      if (lane >= PQ_ROUND || i >= tiles) return;
+      const int x = lo + i;
+      int a = 0, b = entries;
+#pragma unroll 1
+      while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        if (s_first[mid] <= x) a = mid;
+        else b = mid;
+      }
+      int first = s_first[a];
+      next.seq = a * run;
+      next.len = run == 1 ? s_len[a] : read_len(next.seq);
+#pragma unroll 1
+      while (x >= first + tiles_in(next.len)) {
+        first += tiles_in(next.len);
+        next.len = read_len(++next.seq);
+      }
+      next.tile = x - first;
+      const int left = next.len - next.tile * PQ_KEYS;
+      next.keys = min(left, 16) | max(0, min(left - 16, 16)) << 8;
+      const int* row = block_table + static_cast<size_t>(next.seq) * max_blocks;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int stretch = min(next.tile * 2 + u, (next.len - 1) >> 4), in = sub_shift >= 0 ? stretch >> sub_shift : stretch / subs;
+        next.row[u] = (stretch - in * subs) * 16;
+        blk[u] = __ldcg(row + in);
+      }
+    };
+    auto place = [&](int i) {               // its rows, and its scales on their way
+      if (lane >= PQ_ROUND || i >= tiles) return;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool good = q8_index_ok(blk[u], num_blocks, status);
+        if (!good) next.keys &= u ? 0xff : 0xff00;
+        const long head = good ? static_cast<long>(blk[u]) * Hkv + kvh : kvh;
+        next.row[u] += static_cast<int>(head * block_size);
+        next.ks[u] = __ldcg(k_scale + head);
+        next.vs[u] = __ldcg(v_scale + head);
+      }
+    };
+    auto note = [&](int i) {
+      if (lane < PQ_ROUND && i < tiles) {
+        int4* n = reinterpret_cast<int4*>(notes + i % PQ_NOTES);
+        n[0] = make_int4(next.seq, next.tile, next.len, next.keys);
+        *reinterpret_cast<float4*>(n + 1) = make_float4(next.ks[0], next.ks[1], next.vs[0], next.vs[1]);
+        *reinterpret_cast<int2*>(n + 2) = make_int2(next.row[0], next.row[1]);
+      }
+      __syncwarp();
+    };
+    auto bring = [&](int i, int keys, int row0, int row1) {       // one lane; nothing of the stage is read any more
+      uint64_t* full = &s_full[warp][i % STAGES];
+      uint8_t* to = ring + i % STAGES * S::STAGE;
+      const int bytes = ((keys & 0xff) ? 2 * S::STRETCH : 0) + ((keys >> 8) ? 2 * S::STRETCH : 0);
+      mbar_expect_tx(full, bytes);
+      if (keys & 0xff) {
+        tma_load_2d(to, &k_map, 0, row0, full);
+        tma_load_2d(to + 2 * S::STRETCH, &v_map, 0, row0, full);
+      }
+      if (keys >> 8) {
+        tma_load_2d(to + S::STRETCH, &k_map, 0, row1, full);
+        tma_load_2d(to + 3 * S::STRETCH, &v_map, 0, row1, full);
+      }
+    };
+    find(lane);
+    place(lane);
+    if (lane < min(STAGES, tiles)) bring(lane, next.keys, next.row[0], next.row[1]);
+    note(lane);
+
+    int piece_lo = notes[0].tile;
     // this lane's bytes of a stretch: of the keys g and g + 8, and of the values 2t, 2t + 1 (and 8 further)
     const int k_at[2] = {HD == 32 ? pq_piece_at<HD>(g, t >> 1) + (t & 1) * 8 : pq_piece_at<HD>(g, HD == 128 ? 2 * t : t),
                          HD == 128 ? pq_piece_at<HD>(g, 2 * t + 1) : 0};
@@ -313,6 +320,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     uint32_t qf[NT][JT][2];
     float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4], unit, per_unit;
     bool fresh = true;
+#pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
       if (fresh) {
         fresh = false;
@@ -322,7 +330,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         for (int n = 0; n < NT; ++n) {
           uint32_t raw[JT * 2], top = 0;
           const int head = n * 8 + g;
-          const __nv_bfloat16* row = q + static_cast<size_t>(seq) * ldq + (kvh * G + head) * HD + t * (HD / 4);
+          const __nv_bfloat16* row = q + static_cast<size_t>(notes[i % PQ_NOTES].seq) * ldq + (kvh * G + head) * HD + t * (HD / 4);
 #pragma unroll
           for (int v = 0; v < JT * 2 / 4; ++v) {
             const uint4 x = head < G ? __ldcg(reinterpret_cast<const uint4*>(row) + v) : make_uint4(0, 0, 0, 0);
@@ -365,9 +373,9 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         s_abort = 1;
         break;
       }
-      const int4 n0 = *reinterpret_cast<const int4*>(&s_note[warp][i % PQ_NOTES]);
-      const float4 n1 = *reinterpret_cast<const float4*>(s_note[warp][i % PQ_NOTES].ks);
-      const int tile = n0.x, len = n0.y, keys[2] = {n0.z, n0.w};
+      const int4 n0 = *reinterpret_cast<const int4*>(notes + i % PQ_NOTES);
+      const float4 n1 = *reinterpret_cast<const float4*>(notes[i % PQ_NOTES].ks);
+      const int seq = n0.x, tile = n0.y, len = n0.z, keys[2] = {n0.w & 0xff, n0.w >> 8};
       const float ks[2] = {n1.x, n1.y};
       float vs[2] = {n1.z, n1.w};
 
@@ -404,8 +412,15 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) pq_take<VW * 4>(vr[u][r], codes + (2 + u) * S::STRETCH + (r >> 1) * 8 * HD + v_at[r & 1]);
+      const int ahead = i + STAGES;
+      if (ahead % PQ_ROUND == PQ_ROUND / 2) find(ahead + PQ_ROUND / 2 + lane);
+      if (ahead % PQ_ROUND == PQ_ROUND * 3 / 4) place(ahead + PQ_ROUND / 4 + lane);
+      if (ahead % PQ_ROUND == 0) note(ahead + lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[warp][stage]);
+      if (lane == 0 && ahead < tiles) {
+        const PqNote* n = notes + ahead % PQ_NOTES;
+        bring(ahead, n->keys, n->row[0], n->row[1]);
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -531,41 +546,35 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const int head = n * 8 + 2 * t + x;
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-              acc[n][j][x] *= unit;
-              acc[n][j][2 + x] *= unit;
-            }
+            const float f = whole ? (sum == 0.f ? 0.f : unit * rcp_approx(sum)) : unit;
             if (whole) {
               if (head < G) {
                 __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
 #pragma unroll
                 for (int j = 0; j < JT; j += 2)
-                  pq_store4(o_row + 2 * j, make_float4(acc[n][j][x], acc[n][j][2 + x], acc[n][j + 1][x], acc[n][j + 1][2 + x]), sum);
+                  pq_store4(o_row + 2 * j, acc[n][j][x] * f, acc[n][j][2 + x] * f, acc[n][j + 1][x] * f, acc[n][j + 1][2 + x] * f);
               }
             } else {
               float* dst = piece + head * HD + g * (HD / 8);
 #pragma unroll
               for (int j = 0; j < JT; j += 2)
-                *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(acc[n][j][x], acc[n][j][2 + x], acc[n][j + 1][x], acc[n][j + 1][2 + x]);
+                *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(acc[n][j][x] * f, acc[n][j][2 + x] * f, acc[n][j + 1][x] * f, acc[n][j + 1][2 + x] * f);
               if (g == 0) {
                 piece[HEADS * HD + head] = m[n][x];
                 piece[HEADS * HD + HEADS + head] = sum;
               }
             }
           }
-        if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, first, piece_lo, tile + 1};
-        first = lo + i + 1;                   // the next sequence begins with the next tile
-        piece_lo = 0;
+        if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, lo + i - tile, piece_lo, tile + 1};
+        piece_lo = 0;                         // the next sequence begins with the next tile
         fresh = true;
-        if (i + 1 < tiles) do ++seq; while (length(seq) == 0);
       }
     }
   }
   pdl_launch_dependents();
   __syncthreads();
   if (s_abort) {                              // no copy may outlive the CTA
-    if (warp < PQ_WARPS && lane < STAGES) mbar_wait_timed(&s_full[warp][lane], 0, 100), mbar_wait_timed(&s_full[warp][lane], 1, 100);
+    if (lane < STAGES) mbar_wait_timed(&s_full[warp][lane], 0, 100), mbar_wait_timed(&s_full[warp][lane], 1, 100);
     return;
   }
 
@@ -573,7 +582,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   auto piece_of = [&](int p) {
     return reinterpret_cast<const float*>(p & 1 ? rings + (p >> 1) * S::RING : rings + PQ_WARPS * S::RING + (p >> 1) * S::PIECE);
   };
-  const int slot_floats = pq_piece_floats(G, HD), items = G * (HD / 4);
+  const int slot_floats = pq_piece_floats(G, HD), items = G * (HD / 8);           // a thread adds up 8 values of a head
   // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
   auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
   // what holds nothing has no reference, or has met a value that is not a number
@@ -596,36 +605,31 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     }
     __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + kvh * G * HD;
     float* to = slot(share, front.lo == 0);
-#pragma unroll 2
+#pragma unroll 1
     for (int idx = tid; idx < items; idx += PQ_THREADS) {
-      const int r = idx / (HD / 4);
-      float m[PQ_WARPS], l[PQ_WARPS], top = -INFINITY, sum = 0.f;
-      float4 v[PQ_WARPS], o = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int r = idx / (HD / 8);
+      float m[PQ_WARPS], l[PQ_WARPS], top = -INFINITY;
+      PqSum sum{};
 #pragma unroll
       for (int w = 0; w < PQ_WARPS; ++w) {
-        m[w] = -INFINITY;
-        l[w] = 0.f;
-        v[w] = o;
-        if (from[w]) {
-          m[w] = from[w][HEADS * HD + r];
-          l[w] = from[w][HEADS * HD + HEADS + r];
-          v[w] = *reinterpret_cast<const float4*>(from[w] + idx * 4);
-        }
+        m[w] = from[w] ? from[w][HEADS * HD + r] : -INFINITY;
+        l[w] = from[w] ? from[w][HEADS * HD + HEADS + r] : 0.f;
         top = fmaxf(top, m[w]);
       }
 #pragma unroll
-      for (int w = 0; w < PQ_WARPS; ++w) {
-        const float f = weight(m[w], l[w], top);
-        sum = fmaf(l[w], f, sum);
-        o = make_float4(fmaf(v[w].x, f, o.x), fmaf(v[w].y, f, o.y), fmaf(v[w].z, f, o.z), fmaf(v[w].w, f, o.w));
-      }
+      for (int w = 0; w < PQ_WARPS; ++w)
+        if (from[w]) {
+          const float4* v = reinterpret_cast<const float4*>(from[w]) + idx * 2;
+          sum.add(v[0], v[1], l[w], weight(m[w], l[w], top));
+        }
       if (whole) {
-        pq_store4(o_row + idx * 4, o, sum);
+        sum.store(o_row + idx * 8);
       } else {
-        __stcg(reinterpret_cast<float4*>(to + idx * 4), o);
-        if (idx * 4 == r * HD) {
+        __stcg(reinterpret_cast<float4*>(to) + idx * 2, sum.a);
+        __stcg(reinterpret_cast<float4*>(to) + idx * 2 + 1, sum.b);
+        if (idx * 8 == r * HD) {
           __stcg(to + G * HD + r, top);
-          __stcg(to + G * HD + G + r, sum);
+          __stcg(to + G * HD + G + r, sum.l);
         }
       }
     }
@@ -639,40 +643,38 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       __syncthreads();
       if (s_done) {
-#pragma unroll 2
+        const size_t stride = static_cast<size_t>(Hkv) * 2 * slot_floats;
+        const float* part0 = slot(sh0, false);               // the first part lies behind it, the others there
+#pragma unroll 1
         for (int idx = tid; idx < items; idx += PQ_THREADS) {
-          const int r = idx / (HD / 4);
-          float top = -INFINITY, sum = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          const int r = idx / (HD / 8);
+          float top = -INFINITY;
+          PqSum sum{};
+#pragma unroll 1
           for (int q0 = 0; q0 < parts; q0 += 8) {            // eight parts' loads in flight
             float m[8], l[8], now = top;
-            float4 v[8];
+            float4 a[8], b[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               m[j] = -INFINITY;
               l[j] = 0.f;
-              v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+              a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
               if (q0 + j < parts) {
-                const float* sl = slot(sh0 + q0 + j, q0 + j == 0);
+                const float* sl = part0 + (q0 + j) * stride + (q0 + j == 0 ? slot_floats : 0);
                 m[j] = __ldcg(sl + G * HD + r);
                 l[j] = __ldcg(sl + G * HD + G + r);
-                v[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx);
+                a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
+                b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
               }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
-            const float c = top == -INFINITY ? 1.f : pq_exp2(top - now);
+            sum.scale(top == -INFINITY ? 1.f : pq_exp2(top - now));
             top = now;
-            sum *= c;
-            o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float f = weight(m[j], l[j], now);
-              sum = fmaf(l[j], f, sum);
-              o = make_float4(fmaf(v[j].x, f, o.x), fmaf(v[j].y, f, o.y), fmaf(v[j].z, f, o.z), fmaf(v[j].w, f, o.w));
-            }
+            for (int j = 0; j < 8; ++j) sum.add(a[j], b[j], l[j], weight(m[j], l[j], now));
           }
-          pq_store4(o_row + idx * 4, o, sum);
+          sum.store(o_row + idx * 8);
         }
         if (tid == 0) count[seq * Hkv + kvh] = 0;            // as the next launch expects it
       }
