@@ -26,6 +26,7 @@ constexpr int PQ_MIN_TILES = PQ_WARPS;   // tiles of a CTA at least: one per war
 constexpr int PQ_ENTRIES = 1024;         // of a CTA's list of where sequences begin
 constexpr int PQ_ROUND = 16;             // tiles that a warp looks up at a time
 constexpr int PQ_NOTES = 2 * PQ_ROUND;   // and keeps noted: those in use and the next
+constexpr int PQ_BATCH = 12;             // parts of a sequence that are added up at a time
 constexpr float PQ_SLACK = 8.f;          // how far (in powers of two) a score may pass the reference before that moves
 
 __host__ __device__ constexpr int pq_heads(int G) { return G > 8 ? 16 : 8; }
@@ -110,6 +111,11 @@ __device__ __forceinline__ uint32_t pq_half2(float a, float b) {
 __device__ __forceinline__ void pq_store4(__nv_bfloat16* dst, float a, float b, float c, float d) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
 }
+template <int N>
+struct PqInt {
+  static constexpr int value = N;
+};
+
 // A weighted sum of pieces: eight values of a head, and the sum of its weights.
 struct PqSum {
   float4 a, b;
@@ -163,9 +169,10 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD, HEADS);
   extern __shared__ uint8_t pq_smem_raw[];
   uint8_t* rings = pq_smem_raw + (1024 - (smem_u32(pq_smem_raw) & 1023));
-  __shared__ int s_warp[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES], s_done;
+  __shared__ int s_warp[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES];
   __shared__ volatile int s_abort;
   __shared__ PqPiece s_piece[2 * PQ_WARPS];
+  __shared__ int4 s_part[2];                // sequences that the CTA leaves a part of: number, first share, parts, 1: it is the last
   __shared__ PqNote s_note[PQ_WARPS][PQ_NOTES];
   __shared__ __align__(8) uint64_t s_full[PQ_WARPS][STAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -173,7 +180,10 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     mbar_init(&s_full[0][0] + tid, 1);
     fence_mbar_init();
   }
-  if (tid < 2 * PQ_WARPS) s_piece[tid].seq = -1;
+  if (tid < 2 * PQ_WARPS) {
+    s_piece[tid].seq = -1;
+    if (tid < 2) s_part[tid] = make_int4(0, 0, 0, 0);
+  }
   if (tid == PQ_THREADS - 1) {
     s_abort = 0;
     tma_prefetch_desc(&k_map);
@@ -305,40 +315,45 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         tma_load_2d(to + 3 * S::STRETCH, &v_map, 0, row1, full);
       }
     };
-    find(lane);
-    place(lane);
-    if (lane < min(STAGES, tiles)) bring(lane, next.keys, next.row[0], next.row[1]);
-    note(lane);
-
-    int piece_lo = notes[0].tile;
     // this lane's bytes of a stretch: of the keys g and g + 8, and of the values 2t, 2t + 1 (and 8 further)
     const int k_at[2] = {HD == 32 ? pq_piece_at<HD>(g, t >> 1) + (t & 1) * 8 : pq_piece_at<HD>(g, HD == 128 ? 2 * t : t),
                          HD == 128 ? pq_piece_at<HD>(g, 2 * t + 1) : 0};
     const int v_piece = HD == 128 ? g : HD == 64 ? g >> 1 : g >> 2, v_rest = HD == 128 ? 0 : HD == 64 ? (g & 1) * 8 : (g & 3) * 4;
     const int v_at[2] = {pq_piece_at<HD>(2 * t, v_piece) + v_rest, pq_piece_at<HD>(2 * t + 1, v_piece) + v_rest};
 
-    uint32_t qf[NT][JT][2];
+    uint32_t q_raw[NT][JT * 2], qf[NT][JT][2];
     float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4], unit, per_unit;
+    auto request_q = [&](int seq) {         // heads g (and g + 8), hd / 4 values: those that the lane holds of a key, in the same order
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int head = n * 8 + g;
+        const uint4* row = reinterpret_cast<const uint4*>(q + static_cast<size_t>(seq) * ldq + (kvh * G + head) * HD + t * (HD / 4));
+#pragma unroll
+        for (int v = 0; v < JT / 2; ++v) {
+          const uint4 x = head < G ? __ldcg(row + v) : make_uint4(0, 0, 0, 0);
+          q_raw[n][4 * v] = x.x;
+          q_raw[n][4 * v + 1] = x.y;
+          q_raw[n][4 * v + 2] = x.z;
+          q_raw[n][4 * v + 3] = x.w;
+        }
+      }
+    };
+    find(lane);
+    request_q(__shfl_sync(0xffffffffu, next.seq, 0));
+    place(lane);
+    if (lane < min(STAGES, tiles)) bring(lane, next.keys, next.row[0], next.row[1]);
+    note(lane);
+
+    int piece_lo = notes[0].tile;
     bool fresh = true;
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
       if (fresh) {
         fresh = false;
         unit = per_unit = 0.f;
-        // heads g (and g + 8), hd / 4 values: those that the lane holds of a key, in the same order
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint32_t raw[JT * 2], top = 0;
-          const int head = n * 8 + g;
-          const __nv_bfloat16* row = q + static_cast<size_t>(notes[i % PQ_NOTES].seq) * ldq + (kvh * G + head) * HD + t * (HD / 4);
-#pragma unroll
-          for (int v = 0; v < JT * 2 / 4; ++v) {
-            const uint4 x = head < G ? __ldcg(reinterpret_cast<const uint4*>(row) + v) : make_uint4(0, 0, 0, 0);
-            raw[4 * v] = x.x;
-            raw[4 * v + 1] = x.y;
-            raw[4 * v + 2] = x.z;
-            raw[4 * v + 3] = x.w;
-          }
+          uint32_t(&raw)[JT * 2] = q_raw[n], top = 0;
 #pragma unroll
           for (int v = 0; v < JT * 2; ++v) top = __vmaxu2(top, raw[v] & 0x7fff7fffu);
           top = max(top & 0xffffu, top >> 16);
@@ -566,6 +581,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             }
           }
         if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, lo + i - tile, piece_lo, tile + 1};
+        if (i + 1 < tiles) request_q(notes[(i + 1) % PQ_NOTES].seq);
         piece_lo = 0;                         // the next sequence begins with the next tile
         fresh = true;
       }
@@ -589,6 +605,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : pq_exp2(m - top); };
   const int my_seq = lane < 2 * PQ_WARPS ? s_piece[lane].seq : -1;
   uint32_t todo = __ballot_sync(0xffffffffu, my_seq >= 0);
+#pragma unroll 1
   while (todo) {
     const int p0 = __ffs(todo) - 1, seq = __shfl_sync(0xffffffffu, my_seq, p0);
     const uint32_t mine = __ballot_sync(0xffffffffu, my_seq == seq);
@@ -633,53 +650,63 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
       }
     }
-    if (!whole) {
-      __syncthreads();
-      const int sh0 = front.first / per, parts = (front.first + tiles - 1) / per - sh0 + 1;
-      if (tid == 0) {
-        __threadfence();                                     // of what the CTA wrote before the barrier
-        s_done = atomicAdd(&count[seq * Hkv + kvh], 1) == parts - 1;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_done) {
-        const size_t stride = static_cast<size_t>(Hkv) * 2 * slot_floats;
-        const float* part0 = slot(sh0, false);               // the first part lies behind it, the others there
-#pragma unroll 1
-        for (int idx = tid; idx < items; idx += PQ_THREADS) {
-          const int r = idx / (HD / 8);
-          float top = -INFINITY;
-          PqSum sum{};
-#pragma unroll 1
-          for (int q0 = 0; q0 < parts; q0 += 8) {            // eight parts' loads in flight
-            float m[8], l[8], now = top;
-            float4 a[8], b[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              m[j] = -INFINITY;
-              l[j] = 0.f;
-              a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (q0 + j < parts) {
-                const float* sl = part0 + (q0 + j) * stride + (q0 + j == 0 ? slot_floats : 0);
-                m[j] = __ldcg(sl + G * HD + r);
-                l[j] = __ldcg(sl + G * HD + G + r);
-                a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
-                b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
-            sum.scale(top == -INFINITY ? 1.f : pq_exp2(top - now));
-            top = now;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum.add(a[j], b[j], l[j], weight(m[j], l[j], now));
-          }
-          sum.store(o_row + idx * 8);
-        }
-        if (tid == 0) count[seq * Hkv + kvh] = 0;            // as the next launch expects it
-      }
-      __syncthreads();                                       // s_done is read before the next part sets it
+    if (!whole && tid == 0) {
+      const int sh0 = front.first / per;
+      s_part[front.lo == 0] = make_int4(seq, sh0, (front.first + tiles - 1) / per - sh0 + 1, 0);
     }
+  }
+  __syncthreads();
+  if (warp < 2 && lane == 0 && s_part[warp].z > 0) {
+    __threadfence();                                         // of what the CTA wrote before the barrier
+    s_part[warp].w = atomicAdd(&count[s_part[warp].x * Hkv + kvh], 1) == s_part[warp].z - 1;
+    __threadfence();
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if (!s_part[k].w) continue;
+    const int seq = s_part[k].x, parts = s_part[k].z;
+    const size_t stride = static_cast<size_t>(Hkv) * 2 * slot_floats;
+    const float* part0 = slot(s_part[k].y, false);           // the first part lies behind it, the others there
+    // parts q0, q0 + 1, ...: their loads in flight together
+    auto add_parts = [&](auto batch, int q0, int idx, PqSum& sum, float& top) {
+      constexpr int N = decltype(batch)::value;
+      const int r = idx / (HD / 8);
+      float m[N], l[N], now = top;
+      float4 a[N], b[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        m[j] = -INFINITY;
+        l[j] = 0.f;
+        a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (q0 + j < parts) {
+          const float* sl = part0 + (q0 + j) * stride + (q0 + j == 0 ? slot_floats : 0);
+          m[j] = __ldcg(sl + G * HD + r);
+          l[j] = __ldcg(sl + G * HD + G + r);
+          a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
+          b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) now = fmaxf(now, m[j]);
+      sum.scale(top == -INFINITY ? 1.f : pq_exp2(top - now));
+      top = now;
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum.add(a[j], b[j], l[j], weight(m[j], l[j], now));
+    };
+#pragma unroll 1
+    for (int idx = tid; idx < items; idx += PQ_THREADS) {
+      float top = -INFINITY;
+      PqSum sum{};
+      if (parts <= 4) {
+        add_parts(PqInt<4>(), 0, idx, sum, top);
+      } else {
+#pragma unroll 1
+        for (int q0 = 0; q0 < parts; q0 += PQ_BATCH) add_parts(PqInt<PQ_BATCH>(), q0, idx, sum, top);
+      }
+      sum.store(out + static_cast<size_t>(seq) * ldo + kvh * G * HD + idx * 8);
+    }
+    if (tid == 0) count[seq * Hkv + kvh] = 0;                // as the next launch expects it
   }
 }
 
