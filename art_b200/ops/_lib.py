@@ -135,11 +135,18 @@ def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(device: int) -> int:
+    """The current stream of a device, without the objects that :func:`stream_ptr` makes."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
 def status_word(device: torch.device | int | None = None) -> torch.Tensor:
+    if type(device) is int and device in _status:
+        return _status[device]
     idx = torch.cuda.current_device() if device is None else torch.device(device).index
     if idx is None:
         idx = torch.cuda.current_device()

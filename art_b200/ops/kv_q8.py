@@ -51,8 +51,8 @@ def check_geometry(dtype: torch.dtype, block_size: int, hd: int) -> None:
         raise ValueError(f"head dim {hd}: a cache in 8 bits takes {', '.join(map(str, HEAD_DIMS))}")
 
 
-def _check_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
-    """(blocks, Hkv, block_size, hd) of a cache that is one."""
+def _check_cache(k_cache, v_cache, k_scale, v_scale) -> None:
+    """Says what is wrong with a cache."""
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} {k_cache.dtype} and v_cache {tuple(v_cache.shape)} {v_cache.dtype} differ "
                          "or are not [blocks, Hkv, block_size, hd]")
@@ -63,39 +63,59 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int
             raise ValueError(f"{name} must be contiguous fp32 [{nb}, {hkv}]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be contiguous")
-    return nb, hkv, bs, hd
+    raise ValueError(f"a cache of {nb} blocks and {hkv} kv heads")
 
 
-def _check_rows(name: str, x: torch.Tensor, cols: tuple, width: int) -> None:
-    """``x`` [rows, ld] bf16 that holds ``width`` columns from each of ``cols`` on, in pieces of 16 bytes."""
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or (x.shape[1] > 1 and x.stride(1) != 1):
+def _geometry(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int, int]:
+    """(blocks, Hkv, block_size, hd, kind) of a cache that is one.  These checks run before every launch, and a launch takes the
+    GPU a few microseconds: what is in order is found so with as few calls as there are conditions."""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    kind = KINDS.get(dtype)
+    if len(shape) == 4 and kind is not None and v_cache.shape == shape and v_cache.dtype is dtype:
+        nb, hkv, bs, hd = shape
+        scales = (nb, hkv)
+        if (nb > 0 and hkv > 0 and bs > 0 and bs % 16 == 0 and hd in HEAD_DIMS and k_scale.shape == scales and v_scale.shape == scales
+                and k_scale.dtype is v_scale.dtype is torch.float32 and k_cache.is_contiguous() and v_cache.is_contiguous()
+                and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            return nb, hkv, bs, hd, kind
+    _check_cache(k_cache, v_cache, k_scale, v_scale)
+
+
+def _rows(name: str, x: torch.Tensor, lo: int, hi: int, width: int) -> tuple[int, int]:
+    """(rows, row stride) of ``x`` [rows, ld] bf16 that holds ``width`` columns from ``lo`` and from ``hi`` on, in pieces of 16 bytes."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 2 or x.dtype is not torch.bfloat16 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{name} must be bf16 [rows, columns] with unit inner stride")
-    if any(c < 0 or c % 8 or c + width > x.shape[1] for c in cols):
-        raise ValueError(f"{name} [{x.shape[0]}, {x.shape[1]}] does not hold {width} columns at {cols}, multiples of 8")
-    if x.shape[0] > 1 and x.stride(0) % 8 or x.data_ptr() % 16:
+    if lo < 0 or hi < 0 or lo % 8 or hi % 8 or max(lo, hi) + width > shape[1]:
+        raise ValueError(f"{name} [{shape[0]}, {shape[1]}] does not hold {width} columns at {lo} and {hi}, multiples of 8")
+    if (stride[0] % 8 and shape[0] > 1) or x.data_ptr() % 16:
         raise ValueError(f"{name}: rows must begin on 16 bytes")
+    return shape[0], stride[0] if shape[0] > 1 else shape[1] + -shape[1] % 8
 
 
-def _check_index(name: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+def _index(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}]")
 
 
-def _device(*tensors: torch.Tensor) -> torch.device:
-    dev = tensors[0].device
-    if dev.type != "cuda" or any(t.device != dev for t in tensors):
-        raise ValueError(f"tensors of one CUDA device are needed: {', '.join(sorted({str(t.device) for t in tensors}))}")
+def _device(*tensors: torch.Tensor) -> int:
+    """Number of the CUDA device that all tensors lie on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"tensors of one CUDA device are needed: {', '.join(sorted({str(t.device) for t in tensors}))}")
     return dev
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """On the current stream of ``dev``, whichever device is current."""
-    what = name.removeprefix("artb_")
-    if dev.index == torch.cuda.current_device():
-        _lib.check_rc(_f(name)(*args, _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr()), what)
-    else:
+def _launch(dev: int, name: str, *args) -> None:
+    """On the current stream of device ``dev``, whichever device is current."""
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            _lib.check_rc(_f(name)(*args, _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr()), what)
+            return _launch(dev, name, *args)
+    rc = _f(name)(*args, _lib.status_word(dev).data_ptr(), _lib.raw_stream(dev))
+    if rc:
+        _lib.check_rc(rc, name.removeprefix("artb_"))
+    _lib.LAUNCHES += 1
 
 
 def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -107,39 +127,41 @@ def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k
     The scale of a block and head is the least power of two that takes the largest value written to it into the range of the
     codes.  A row at a block's first place starts the block anew.  Rows at later places can only raise the scale, and then what
     the block holds already is rounded once more.  A value that is not finite makes the scale NaN until the block starts anew."""
-    nb, hkv, bs, hd = _check_cache(k_cache, v_cache, k_scale, v_scale)
-    _check_rows("qkv", qkv, (k_col, v_col), hkv * hd)
-    _check_index("slot", slot, qkv.shape[0])
+    nb, hkv, bs, hd, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
+    n, ld = _rows("qkv", qkv, k_col, v_col, hkv * hd)
+    _index("slot", slot, n)
     dev = _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_write_q8", _lib.ptr(qkv), qkv.stride(0), k_col, v_col, _lib.ptr(slot), _lib.ptr(k_cache), _lib.ptr(v_cache),
-            _lib.ptr(k_scale), _lib.ptr(v_scale), qkv.shape[0], hkv, hd, bs, nb, KINDS[k_cache.dtype])
+    _launch(dev, "artb_kv_write_q8", qkv.data_ptr(), ld, k_col, v_col, slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, hd, bs, nb, kind)
 
 
 def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot: torch.Tensor,
                dst: torch.Tensor, k_col: int, v_col: int) -> None:
     """The cached keys and values at ``slot`` (int32 [n]) as bf16 into the k and v columns of ``dst[:n]``; zeros where negative."""
-    nb, hkv, bs, hd = _check_cache(k_cache, v_cache, k_scale, v_scale)
-    _check_rows("dst", dst, (k_col, v_col), hkv * hd)
-    if abs(k_col - v_col) < hkv * hd or (dst.shape[0] > 1 and dst.stride(0) < max(k_col, v_col) + hkv * hd):
+    nb, hkv, bs, hd, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
+    have, ld = _rows("dst", dst, k_col, v_col, hkv * hd)
+    if abs(k_col - v_col) < hkv * hd or ld < max(k_col, v_col) + hkv * hd:
         raise ValueError("the columns of keys and values, or the rows of dst, overlap")
     n = slot.numel()
-    _check_index("slot", slot, n)
-    if n > dst.shape[0]:
-        raise ValueError(f"{n} slots for {dst.shape[0]} rows")
+    _index("slot", slot, n)
+    if n > have:
+        raise ValueError(f"{n} slots for {have} rows")
     dev = _device(dst, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_rows_q8", _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(slot), n,
-            _lib.ptr(dst), dst.stride(0), k_col, v_col, hkv, hd, bs, nb, KINDS[k_cache.dtype])
+    _launch(dev, "artb_kv_rows_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slot.data_ptr(), n,
+            dst.data_ptr(), ld, k_col, v_col, hkv, hd, bs, nb, kind)
 
 
 @functools.lru_cache(maxsize=1024)
-def _decode_bytes(n: int, Hq: int, Hkv: int, hd: int, device: int | None) -> int:
+def _decode_bytes(n: int, Hq: int, Hkv: int, hd: int, device: int) -> int:
     with torch.cuda.device(device):
         return _f("artb_paged_decode_q8_bytes")(n, Hq, Hkv, hd)
 
 
 def decode_q8_workspace(n: int, Hq: int, Hkv: int, hd: int, device) -> torch.Tensor:
     """Workspace of :func:`paged_decode_q8` for up to ``n`` sequences; one call at a time may use it."""
-    return torch.zeros(_decode_bytes(n, Hq, Hkv, hd, torch.device(device).index), dtype=torch.uint8, device=device)
+    dev = torch.device(device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    return torch.zeros(_decode_bytes(n, Hq, Hkv, hd, index), dtype=torch.uint8, device=dev)
 
 
 def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -147,23 +169,20 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     ws: torch.Tensor) -> torch.Tensor:
     """Attention of one token per sequence over the first ``ctx_len`` cached tokens: q bf16 [n, >= Hq*hd] (row stride arbitrary),
     ``block_table`` int32 [n, width], ``ctx_len`` int32 [n] (0: the row becomes zeros); out bf16 [n, >= Hq*hd]."""
-    nb, hkv, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
-    if (hkv, d) != (Hkv, hd) or Hq <= 0 or Hq % Hkv or Hq // Hkv > 16:
+    nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
+    if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > 16 * Hkv:
         raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
-    _check_rows("q", q, (0,), Hq * hd)
-    _check_rows("out", out, (0,), Hq * hd)
-    n = q.shape[0]
-    if out.shape[0] != n or (n > 1 and out.stride(0) < Hq * hd):
+    n, ldq = _rows("q", q, 0, 0, Hq * hd)
+    m, ldo = _rows("out", out, 0, 0, Hq * hd)
+    if m != n or ldo < Hq * hd:
         raise ValueError(f"out must have {n} rows that do not overlap")
-    _check_index("ctx_len", ctx_len, n)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1 \
-            or not block_table.is_contiguous():
+    _index("ctx_len", ctx_len, n)
+    table = block_table.shape
+    if block_table.dtype is not torch.int32 or len(table) != 2 or table[0] != n or table[1] < 1 or not block_table.is_contiguous():
         raise ValueError(f"block_table must be contiguous int32 [{n}, width]")
     dev = _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
-    need = _decode_bytes(n, Hq, Hkv, hd, dev.index) if n else 0
-    if ws.numel() * ws.element_size() < need or not ws.is_contiguous():
-        raise ValueError(f"workspace of {ws.numel() * ws.element_size()} bytes, {need} needed in a row")
-    _launch(dev, "artb_paged_decode_q8", _lib.ptr(q), q.stride(0), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale),
-            _lib.ptr(v_scale), _lib.ptr(block_table), block_table.shape[1], _lib.ptr(ctx_len), bs, n, Hq, Hkv, hd, _lib.ptr(out),
-            out.stride(0), _lib.ptr(ws), nb, KINDS[k_cache.dtype])
+    if n and (ws.nbytes < _decode_bytes(n, Hq, Hkv, hd, dev) or not ws.is_contiguous()):
+        raise ValueError(f"workspace of {ws.nbytes} bytes, {_decode_bytes(n, Hq, Hkv, hd, dev)} needed in a row")
+    _launch(dev, "artb_paged_decode_q8", q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), table[1], ctx_len.data_ptr(), bs, n, Hq, Hkv, hd, out.data_ptr(), ldo, ws.data_ptr(), nb, kind)
     return out
