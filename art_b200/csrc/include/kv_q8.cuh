@@ -40,7 +40,7 @@ __device__ __forceinline__ int q8_exponent(uint32_t amax_bits) {
   return e < Q8_LEAST_EXP ? Q8_LEAST_EXP : e;
 }
 
-// Four values, already divided by their scale, to four codes: nearest, ties to even.
+// Four values, already divided by their scale and so within the codes' range, to four codes: nearest, ties to even.
 template <int KIND>
 __device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float d) {
   if (KIND == Q8_E4M3) {
@@ -48,7 +48,9 @@ __device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float 
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   }
-  const uint32_t x = __float2int_rn(a), y = __float2int_rn(b), z = __float2int_rn(c), w = __float2int_rn(d);
+  // beside 1.5 * 2^23 the last bit of a float is 1: the sum is rounded to a whole number, whose low byte is the code
+  constexpr float ONES = 12582912.f;
+  const uint32_t x = __float_as_uint(a + ONES), y = __float_as_uint(b + ONES), z = __float_as_uint(c + ONES), w = __float_as_uint(d + ONES);
   return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 

@@ -18,144 +18,182 @@
 
 namespace artb {
 
-// A warp per (run of rows, kv head, keys or values).  A run is a stretch of neighbouring rows whose slots are neighbours in
-// one block; the warps of a CTA look for runs that begin among its ROWS rows and follow them to their ends.
-// A lane holds 8 values of a row: HD / 8 lanes to a row, 16 rows at a time in registers.
-constexpr int KW_BATCH = 16;
+// A run is a stretch of neighbouring rows whose slots are neighbours in one block.  A warp takes a run's part for one kv head, of
+// keys or of values: it looks for the runs that begin among its ROWS rows and follows them to their ends.  A lane holds 8 values
+// of a row, HD / 8 lanes to a row, ITERS * 32 * 8 / HD rows at a time in registers; longer runs are read twice.  FULL: the rows are a multiple of that.
+template <int KIND, int HD, int ITERS, bool FULL>
+__device__ __forceinline__ void kw_run(const __nv_bfloat16* x, int ld, int n, int at, int block_size, uint8_t* codes, float* sp) {
+  constexpr int LPR = HD / 8, RPI = 32 / LPR, BATCH = ITERS * RPI;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, c = (lane % LPR) * 8;
+  const float held = __ldcg(sp);
+  uint4 raw[ITERS];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int r = first + i * RPI + sub;
+      raw[i] = FULL || r < n ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(r) * ld + c) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  // largest |value|: the bits of bf16 magnitudes order like integers, two at a time
+  uint32_t top = 0;
+  for (int first = 0; first < n; first += BATCH) {
+    load(first);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      top = __vmaxu2(top, raw[i].x & 0x7fff7fffu);
+      top = __vmaxu2(top, raw[i].y & 0x7fff7fffu);
+      top = __vmaxu2(top, raw[i].z & 0x7fff7fffu);
+      top = __vmaxu2(top, raw[i].w & 0x7fff7fffu);
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
 
+  const float mine = q8_pow2(q8_exponent<KIND>(top < 0x7f80u ? top << 16 : 0u));
+  const bool anew = at == 0, bad = top >= 0x7f80u || (!anew && !(held <= 3.0e38f));         // not finite
+  const float to = anew ? mine : fmaxf(held, mine), inv = 1.f / to;                         // exact: a power of two
+  __syncwarp();                              // every lane has the old scale
+  if (lane == 0) *sp = bad ? __int_as_float(0x7fc00000) : to;
+  if (!bad && !anew && to > held) {
+    const float down = held * inv;
+    for (int v = lane; v < block_size * (HD / 16); v += 32) {
+      const int place = v / (HD / 16);
+      if (place >= at && place < at + n) continue;
+      uint4* p = reinterpret_cast<uint4*>(codes) + v;
+      uint4 old = *p;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&old);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        q8_decode4<KIND>(w[j], f);
+        w[j] = q8_encode4<KIND>(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
+      }
+      *p = old;
+    }
+  }
+  for (int first = 0; first < n; first += BATCH) {
+    if (n > BATCH) load(first);              // else the only batch is still in registers
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int r = first + i * RPI + sub;
+      if (!FULL && r >= n) continue;
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = __uint_as_float(w[j] << 16) * inv;
+        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
+      }
+      uint2 out = make_uint2(q8_encode4<KIND>(f[0], f[1], f[2], f[3]), q8_encode4<KIND>(f[4], f[5], f[6], f[7]));
+      if (bad) out = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(codes + static_cast<size_t>(at + r) * HD + c) = out;
+    }
+  }
+}
+
+// ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 3.3 us, 4.6 with four to a warp, 12 with
+// sixteen), a block's worth where prompts bring many (14,000 rows: 20 us, 26 with four to a warp, 64 with one).
 template <int KIND, int HD, int ROWS>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 6)
 kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int v_col, const int* __restrict__ slot,
                    uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int M, int Hkv, int block_size,
-                   long num_blocks, int* status) {
-  constexpr int LPR = HD / 8, RPI = 32 / LPR, ITERS = KW_BATCH / RPI;
+                   int block_shift, long num_blocks, int* status) {
+  static_assert(ROWS <= 16, "a warp sees 32 rows at once, and a run of 16 to its end");
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, part = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, part = blockIdx.y * 4 + (threadIdx.x >> 5), row0 = blockIdx.x * ROWS;
   if (part >= 2 * Hkv) return;
   const bool is_v = part >= Hkv;
   const int h = is_v ? part - Hkv : part;
   const __nv_bfloat16* x = qkv + (is_v ? v_col : k_col) + h * HD;
   uint8_t* cache = is_v ? v_cache : k_cache;
   float* scales = is_v ? v_scale : k_scale;
-  const int row0 = blockIdx.x * ROWS, sub = lane / LPR, c = (lane % LPR) * 8;
 
-  bool starts = false;
-  if (lane < ROWS && row0 + lane < M) {
-    const int r = row0 + lane, s = slot[r];
-    starts = s >= 0 && (r == 0 || s % block_size == 0 || slot[r - 1] != s - 1);
-  }
-  for (uint32_t todo = __ballot_sync(0xffffffffu, starts); todo; todo &= todo - 1) {
-    const int r0 = row0 + __ffs(todo) - 1, s0 = slot[r0];
+  const int s = row0 + lane < M ? slot[row0 + lane] : -1;
+  int prev = __shfl_up_sync(0xffffffffu, s, 1);
+  if (lane == 0) prev = row0 > 0 ? slot[row0 - 1] : -1;
+  const int blk = s < 0 ? 0 : block_shift >= 0 ? s >> block_shift : s / block_size;
+  const bool goes_on = s > 0 && prev == s - 1 && s != blk * block_size;        // with the run of the row before
+  const uint32_t on = __ballot_sync(0xffffffffu, goes_on);
+  for (uint32_t todo = __ballot_sync(0xffffffffu, lane < ROWS && s >= 0 && !goes_on); todo; todo &= todo - 1) {
+    const int i = __ffs(todo) - 1, s0 = __shfl_sync(0xffffffffu, s, i), block = __shfl_sync(0xffffffffu, blk, i);
     if (!q8_index_ok(s0, num_blocks * block_size, status)) continue;
-    const long block = s0 / block_size;
-    const int at = s0 - static_cast<int>(block) * block_size, most = min(block_size - at, M - r0);
-    int n = 1;
-    while (n < most) {                     // the run's length: 32 rows at a time
-      const int r = r0 + n + lane;
-      const uint32_t on = __ballot_sync(0xffffffffu, n + lane < most && slot[min(r, M - 1)] == s0 + n + lane);
-      const int more = on == 0xffffffffu ? 32 : __ffs(~on) - 1;
-      n += more;
-      if (more < 32) break;
+    const int r0 = row0 + i, at = s0 - block * block_size;
+    const uint32_t ends = ~on & (0xfffffffeu << i);
+    int n = (ends ? __ffs(ends) - 1 : 32) - i;
+    while (!ends) {                          // longer than what is seen: 32 rows at a time
+      const int most = min(block_size - at, M - r0);
+      const uint32_t more = __ballot_sync(0xffffffffu, n + lane < most && slot[min(r0 + n + lane, M - 1)] == s0 + n + lane);
+      n += more == 0xffffffffu ? 32 : __ffs(~more) - 1;
+      if (more != 0xffffffffu) break;
     }
-
-    uint4 raw[ITERS];
-    auto load = [&](int first) {
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        const int r = first + i * RPI + sub;
-        raw[i] = r < n ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(r0 + r) * ld + c) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    // largest |value|: the bits of bf16 magnitudes order like integers, two at a time
-    uint32_t top = 0;
-    for (int first = 0; first < n; first += KW_BATCH) {
-      load(first);
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        top = __vmaxu2(top, raw[i].x & 0x7fff7fffu);
-        top = __vmaxu2(top, raw[i].y & 0x7fff7fffu);
-        top = __vmaxu2(top, raw[i].z & 0x7fff7fffu);
-        top = __vmaxu2(top, raw[i].w & 0x7fff7fffu);
-      }
-    }
-    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-
-    float* sp = scales + block * Hkv + h;
-    const float held = *sp, mine = q8_pow2(q8_exponent<KIND>(top < 0x7f80u ? top << 16 : 0u));
-    const bool anew = at == 0, bad = top >= 0x7f80u || (!anew && !(held <= 3.0e38f));       // not finite
-    const float to = anew ? mine : fmaxf(held, mine), inv = 1.f / to;                       // exact: a power of two
-    uint8_t* codes = cache + (block * Hkv + h) * block_size * HD;
-    __syncwarp();
-    if (lane == 0) *sp = bad ? __int_as_float(0x7fc00000) : to;
-    if (!bad && !anew && to > held) {
-      const float down = held * inv;
-      for (int v = lane; v < block_size * (HD / 4); v += 32) {
-        const int place = v / (HD / 4);
-        if (place >= at && place < at + n) continue;
-        uint32_t* p = reinterpret_cast<uint32_t*>(codes) + v;
-        float f[4];
-        q8_decode4<KIND>(*p, f);
-        *p = q8_encode4<KIND>(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
-      }
-    }
-    for (int first = 0; first < n; first += KW_BATCH) {
-      if (n > KW_BATCH) load(first);       // else the only batch is still in registers
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        const int r = first + i * RPI + sub;
-        if (r >= n) continue;
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[2 * j] = __uint_as_float(w[j] << 16) * inv;
-          f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
-        }
-        uint2 out = make_uint2(q8_encode4<KIND>(f[0], f[1], f[2], f[3]), q8_encode4<KIND>(f[4], f[5], f[6], f[7]));
-        if (bad) out = make_uint2(0, 0);
-        *reinterpret_cast<uint2*>(codes + static_cast<size_t>(at + r) * HD + c) = out;
-      }
+    const long head = static_cast<long>(block) * Hkv + h;
+    uint8_t* codes = cache + head * block_size * HD;
+    const __nv_bfloat16* rows = x + static_cast<size_t>(r0) * ld;
+    if (n * (HD / 8) <= 32) {
+      kw_run<KIND, HD, 1, false>(rows, ld, n, at, block_size, codes, scales + head);
+    } else if (n % 16 == 0) {                // whole blocks, for the most part
+      kw_run<KIND, HD, HD / 16, true>(rows, ld, n, at, block_size, codes, scales + head);
+    } else {
+      kw_run<KIND, HD, HD / 16, false>(rows, ld, n, at, block_size, codes, scales + head);
     }
   }
 }
 
 // The cached keys and values at a list of slots -> k | v columns of dst [n, ld], as bf16 (exact: a code has at most 8 bits);
-// rows with a negative slot become zeros.  A thread takes 16 codes.  Bound by bytes, 1 in and 2 out per value.
-template <int KIND>
+// rows with a negative slot become zeros.  A thread takes 16 codes of the same place in ROWS rows at a time, whose loads are in
+// flight together, and stores them as 32 bytes where the destination allows.  Bound by bytes, 1 in and 2 out per value: 18.9 us
+// for 32,000 rows of 4 heads of 128 (98 MB) with four rows, 20.1 with one; what fits the chip once takes one row: 300 of 2 heads
+// of 64 take 2.1 us, 2.9 with four.
+template <int KIND, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(256)
 kv_rows_q8_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const float* __restrict__ k_scale,
-                  const float* __restrict__ v_scale, const int* __restrict__ slot, long n, __nv_bfloat16* __restrict__ dst, int ld,
-                  int k_col, int v_col, int Hkv, int hd, int block_size, long num_blocks, int* status) {
-  const int half = Hkv * hd / 16, vec = 2 * half;
-  const long total = n * vec;
-  for (long i = blockIdx.x * static_cast<long>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<long>(gridDim.x) * blockDim.x) {
-    const long r = i / vec;
-    int u = static_cast<int>(i - r * vec);
-    const bool is_v = u >= half;
-    u -= is_v ? half : 0;
-    const int h = u * 16 / hd, d = u * 16 - h * hd, s = slot[r];
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    float scale = 0.f;
-    if (s >= 0 && q8_index_ok(s, num_blocks * block_size, status)) {
-      const long head = s / block_size * static_cast<long>(Hkv) + h;
-      raw = *reinterpret_cast<const uint4*>((is_v ? v_cache : k_cache) + (head * block_size + s % block_size) * hd + d);
-      scale = (is_v ? v_scale : k_scale)[head];
-    }
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    uint32_t o[8];
+                  const float* __restrict__ v_scale, const int* __restrict__ slot, int n, __nv_bfloat16* __restrict__ dst, int ld,
+                  int k_col, int v_col, int Hkv, int hd, int block_size, int block_shift, long num_blocks, int* status) {
+  const int half = Hkv * hd / 16;
+  for (int at = threadIdx.x; at < 2 * half; at += blockDim.x) {
+    const bool is_v = at >= half;
+    const int u = (is_v ? at - half : at) * 16, h = u / hd, d = u - h * hd;
+    const uint8_t* cache = (is_v ? v_cache : k_cache) + d;
+    const float* scales = is_v ? v_scale : k_scale;
+    __nv_bfloat16* to = dst + (is_v ? v_col : k_col) + u;
+    for (int r0 = (blockIdx.x * blockDim.y + threadIdx.y) * ROWS; r0 < n; r0 += gridDim.x * blockDim.y * ROWS) {
+      uint4 raw[ROWS];
+      float scale[ROWS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[4];
-      q8_decode4<KIND>(w[j], f);
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0] * scale, f[1] * scale), hi = __floats2bfloat162_rn(f[2] * scale, f[3] * scale);
-      o[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
-      o[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+      for (int j = 0; j < ROWS; ++j) {
+        const int s = r0 + j < n ? slot[r0 + j] : -1;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        scale[j] = 0.f;
+        if (s >= 0 && q8_index_ok(s, num_blocks * block_size, status)) {
+          const int block = block_shift >= 0 ? s >> block_shift : s / block_size;
+          const long head = static_cast<long>(block) * Hkv + h;
+          raw[j] = *reinterpret_cast<const uint4*>(cache + (head * block_size + (s - block * block_size)) * hd);
+          scale[j] = scales[head];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) {
+        if (r0 + j >= n) break;
+        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[4];
+          q8_decode4<KIND>(w[i], f);
+          o[2 * i] = pack_bf16x2(f[0] * scale[j], f[1] * scale[j]);
+          o[2 * i + 1] = pack_bf16x2(f[2] * scale[j], f[3] * scale[j]);
+        }
+        if (WIDE) {
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + static_cast<size_t>(r0 + j) * ld), "r"(o[0]),
+                       "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                       : "memory");
+        } else {
+          uint4* p = reinterpret_cast<uint4*>(to + static_cast<size_t>(r0 + j) * ld);
+          p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
     }
-    uint4* to = reinterpret_cast<uint4*>(dst + r * ld + (is_v ? v_col : k_col) + h * hd + d);
-    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -171,14 +209,17 @@ ARTB_EXPORT int artb_kv_write_q8(const void* qkv, int ld, int k_col, int v_col, 
   if (M <= 0) return 0;
   if (Hkv <= 0 || block_size < 16 || (block_size & 15) || (ld & 7) || (k_col & 7) || (v_col & 7)) return ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return ERR_BAD_ALIGN;
+  const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
 #define ARTB_KW(KIND_, HD_)                                                                                                  \
   if (kind == KIND_ && hd == HD_) {                                                                                          \
     auto go = [&](auto kern, int rows) {                                                                                     \
       return static_cast<int>(launch_kernel(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), 0, st,          \
                                             (const __nv_bfloat16*)qkv, ld, k_col, v_col, slot, (uint8_t*)k_cache,            \
-                                            (uint8_t*)v_cache, k_scale, v_scale, M, Hkv, block_size, num_blocks, status));   \
+                                            (uint8_t*)v_cache, k_scale, v_scale, M, Hkv, block_size, shift, num_blocks, status)); \
     };                                                                                                                       \
-    return go(kv_write_q8_kernel<KIND_, HD_, 1>, 1);                                                                         \
+    if (M <= 256) return go(kv_write_q8_kernel<KIND_, HD_, 1>, 1);                                                           \
+    if (M <= 2048) return go(kv_write_q8_kernel<KIND_, HD_, 4>, 4);                                                          \
+    return go(kv_write_q8_kernel<KIND_, HD_, 16>, 16);                                                                       \
   }
   ARTB_KW(Q8_E4M3, 128) ARTB_KW(Q8_E4M3, 64) ARTB_KW(Q8_E4M3, 32)
   ARTB_KW(Q8_INT8, 128) ARTB_KW(Q8_INT8, 64) ARTB_KW(Q8_INT8, 32)
@@ -192,14 +233,24 @@ ARTB_EXPORT int artb_kv_rows_q8(const void* k_cache, const void* v_cache, const 
   if (n <= 0) return 0;
   if (Hkv <= 0 || hd < 16 || (hd & 15) || block_size < 1 || (ld & 7) || (k_col & 7) || (v_col & 7)) return ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return ERR_BAD_ALIGN;
-  long blocks = (static_cast<long>(n) * (Hkv * hd / 8) + 255) / 256;
-  if (blocks > 148L * 16) blocks = 148L * 16;
+  const int vec = Hkv * hd / 8, bx = vec < 256 ? vec : 256, by = 256 / bx;
+  const bool once = (static_cast<long>(n) + by - 1) / by <= 8L * sm_count();
+  const long blocks = (static_cast<long>(n) + by * (once ? 1 : 4) - 1) / (by * (once ? 1 : 4));
+  const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
+  const bool wide = ((reinterpret_cast<uintptr_t>(dst) & 31) | (ld & 15) | (k_col & 15) | (v_col & 15)) == 0;
   auto go = [&](auto kern) {
-    kern<<<(unsigned)blocks, 256, 0, st>>>((const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, slot, n,
-                                           (__nv_bfloat16*)dst, ld, k_col, v_col, Hkv, hd, block_size, num_blocks, status);
+    kern<<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), dim3(bx, by), 0, st>>>(
+        (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, slot, n, (__nv_bfloat16*)dst, ld, k_col, v_col, Hkv, hd,
+        block_size, shift, num_blocks, status);
     return (int)cudaGetLastError();
   };
-  if (kind == Q8_E4M3) return go(kv_rows_q8_kernel<Q8_E4M3>);
-  if (kind == Q8_INT8) return go(kv_rows_q8_kernel<Q8_INT8>);
+#define ARTB_KR(KIND_)                                                                                                     \
+  if (kind == KIND_) {                                                                                                     \
+    if (once) return wide ? go(kv_rows_q8_kernel<KIND_, 1, true>) : go(kv_rows_q8_kernel<KIND_, 1, false>);                \
+    return wide ? go(kv_rows_q8_kernel<KIND_, 4, true>) : go(kv_rows_q8_kernel<KIND_, 4, false>);                          \
+  }
+  ARTB_KR(Q8_E4M3)
+  ARTB_KR(Q8_INT8)
+#undef ARTB_KR
   return ERR_BAD_SHAPE;
 }
