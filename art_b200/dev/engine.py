@@ -134,7 +134,7 @@ NATIVE_ENGINE_KEYS = frozenset({
     "max_num_batched_tokens", "block_size", "gpu_memory_utilization", "tensor_parallel_size",
     "pipeline_parallel_size", "context_parallel_size", "expert_parallel_size", "data_parallel_size",
     "enable_prefix_caching", "enable_chunked_prefill", "num_scheduler_steps", "enforce_eager",
-    "enable_sleep_mode", "enable_lora", "max_loras", "max_lora_rank", "max_logprobs",
+    "enable_sleep_mode", "kv_cache_dtype", "enable_lora", "max_loras", "max_lora_rank", "max_logprobs",
     "disable_log_stats", "disable_log_requests", "generation_config", "num_gpu_blocks_override",
     "multi_step_stream_outputs",
 })

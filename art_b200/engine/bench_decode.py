@@ -15,7 +15,8 @@ import torch
 
 
 def measure_decode(cfg, device, seqs: int = 256, prompt_len: int = 512, new_tokens: int = 128, loras: int = 4,
-                   runs: int = 3, base=None, tp_group=None, prompt_len_max: int = 0, prefill_runs: int = 0) -> dict:
+                   runs: int = 3, base=None, tp_group=None, prompt_len_max: int = 0, prefill_runs: int = 0,
+                   kv_dtype: str = "auto") -> dict:
     """Prefill + decode throughput of one engine replica.  ``tp_group``: the replica spans that process group (every
     rank calls this with the same arguments and gets the same numbers).  ``prompt_len_max`` > ``prompt_len`` draws
     prompt lengths uniformly from [prompt_len, prompt_len_max].  The first ``runs - 1`` passes warm every CUDA-graph
@@ -35,7 +36,7 @@ def measure_decode(cfg, device, seqs: int = 256, prompt_len: int = 512, new_toke
     p_hi = max(prompt_len, prompt_len_max)
     nblocks = seqs * ((p_hi + new_tokens) // bs + 2)
     runner, kv = build_runner(cfg, base, num_blocks=nblocks, block_size=bs, num_slots=seqs, device=dev, lora_cfg=lcfg,
-                              max_loras=max(1, loras), tp_group=tp_group)
+                              max_loras=max(1, loras), tp_group=tp_group, kv_dtype=kv_dtype)
     width = 64
     while width < (p_hi + new_tokens) // bs + 2:
         width *= 2
@@ -91,7 +92,7 @@ def measure_decode(cfg, device, seqs: int = 256, prompt_len: int = 512, new_toke
             torch.distributed.all_reduce(tt, op=torch.distributed.ReduceOp.MAX, group=tp_group)
             t_pre, t_dec = float(tt[0]), float(tt[1])
         res = {"model": cfg.name, "tp": tp, "seqs": seqs, "prompt_len": prompt_len if p_hi == prompt_len else [prompt_len, p_hi],
-               "new_tokens": new_tokens, "loras": loras,
+               "new_tokens": new_tokens, "loras": loras, **({} if kv_dtype == "auto" else {"kv_cache_dtype": kv_dtype}),
                "decode_tok_s": round((gen - gen_at_prefill) / t_dec, 1), "prefill_tok_s": round(n_prompt / t_pre, 1),
                "decode_ms_per_step": round(1e3 * t_dec * seqs / max(1, gen - gen_at_prefill), 3),
                "decode_s": round(t_dec, 4), "prefill_s": round(t_pre, 4), "launches": _lib.LAUNCHES - l0}
@@ -124,6 +125,7 @@ def measure_decode(cfg, device, seqs: int = 256, prompt_len: int = 512, new_toke
 
 def main() -> None:
     from ..models.config import resolve_config
+    from .kv_cache import KV_CACHE_DTYPES
 
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", default="qwen2.5-7b")
@@ -134,6 +136,7 @@ def main() -> None:
     ap.add_argument("--runs", type=int, default=3)
     ap.add_argument("--prompt-len-max", type=int, default=0, help="draw prompt lengths uniformly up to this")
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel replica over all ranks of a torchrun launch")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=list(KV_CACHE_DTYPES))
     a = ap.parse_args()
     group, dev, rank = None, "cuda", 0
     if a.tp > 1:
@@ -147,7 +150,7 @@ def main() -> None:
             raise SystemExit("--tp must equal the number of launched ranks")
         group = dist.group.WORLD
     res = measure_decode(resolve_config(a.model), dev, a.seqs, a.prompt_len, a.new_tokens, a.loras, a.runs, tp_group=group,
-                         prompt_len_max=a.prompt_len_max)
+                         prompt_len_max=a.prompt_len_max, kv_dtype=a.kv_cache_dtype)
     if rank == 0:
         print(json.dumps(res))
     if a.tp > 1:

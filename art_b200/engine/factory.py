@@ -11,7 +11,7 @@ import torch
 from ..models.hybrid import HybridConfig
 from ..models.weights import LoraConfig
 from .engine import Engine
-from .kv_cache import BlockManager, HybridCache, KVCache
+from .kv_cache import BlockManager, HybridCache, KVCache, kv_cache_dtype
 
 
 class UnsupportedPrecision(ValueError):
@@ -20,8 +20,11 @@ class UnsupportedPrecision(ValueError):
 
 def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, block_size: int = 16, num_slots: int = 256,
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, lora_cfg: LoraConfig | None = None,
-                 max_loras: int = 4, tp_group=None, decoder=None, use_arena: bool = False):
-    """``(runner, cache)`` on ``device``.  ``num_slots`` bounds the sequences that hold recurrent state at once."""
+                 max_loras: int = 4, tp_group=None, decoder=None, use_arena: bool = False,
+                 kv_dtype: str | torch.dtype | None = None):
+    """``(runner, cache)`` on ``device``.  ``num_slots`` bounds the sequences that hold recurrent state at once.  ``kv_dtype``: the
+    cache's number format (``kv_cache.KV_CACHE_DTYPES``; None: that of the model)."""
+    cache_dtype = kv_cache_dtype(kv_dtype)
     dev = torch.device(device)
     if dev.type == "cuda" and dev.index is None:       # the engine's stepping thread selects it by number
         dev = torch.device("cuda", torch.cuda.current_device())
@@ -30,6 +33,8 @@ def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, 
 
         if tp_group is not None and torch.distributed.get_world_size(tp_group) > 1:
             raise ValueError("hybrid models run on one GPU per replica")
+        if cache_dtype != torch.bfloat16:
+            raise ValueError("hybrid models keep their caches in the model's number format")
         kv = HybridCache(cfg, num_blocks, block_size, num_slots, dev, dtype)
         return HybridRunner(cfg, kv, base, device=dev, dtype=dtype), kv
     from .runner import NativeRunner
@@ -37,7 +42,7 @@ def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, 
     if dtype != torch.bfloat16:
         raise UnsupportedPrecision(f"{cfg.family} models run in bfloat16")
     tp = 1 if tp_group is None else torch.distributed.get_world_size(tp_group)
-    args = (cfg.num_layers, num_blocks, block_size, cfg.num_kv_heads // tp, cfg.head_dim, dev)
+    args = (cfg.num_layers, num_blocks, block_size, cfg.num_kv_heads // tp, cfg.head_dim, dev, cache_dtype)
     try:
         kv = KVCache(*args, use_arena=use_arena)
     except RuntimeError:   # no VMM support: plain tensors; Engine.sleep() then drops the captured graphs
@@ -48,18 +53,19 @@ def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, 
                         tp_group=tp_group), kv
 
 
-def cache_bytes(cfg, block_size: int, tp: int = 1) -> tuple[int, int]:
+def cache_bytes(cfg, block_size: int, tp: int = 1, kv_dtype: str | torch.dtype | None = None) -> tuple[int, int]:
     """(bytes of one cache block, bytes of one state slot) over all layers."""
     if isinstance(cfg, HybridConfig):
         return max(1, HybridCache.bytes_per_block(cfg, block_size)), HybridCache.bytes_per_slot(cfg)
-    return KVCache.bytes_per_block(cfg.num_layers, block_size, cfg.num_kv_heads // tp, cfg.head_dim), 0
+    return KVCache.bytes_per_block(cfg.num_layers, block_size, cfg.num_kv_heads // tp, cfg.head_dim, kv_cache_dtype(kv_dtype).itemsize), 0
 
 
 def build_engine(cfg, base: dict[str, torch.Tensor], *, num_blocks: int, block_size: int = 16, max_num_seqs: int = 256,
                  max_loras: int = 4, device="cuda", dtype: torch.dtype = torch.bfloat16, lora_cfg: LoraConfig | None = None,
-                 enable_prefix_caching: bool = True, eos_token_id: int | None = None, **engine_kw) -> Engine:
+                 enable_prefix_caching: bool = True, eos_token_id: int | None = None, kv_dtype: str | torch.dtype | None = None,
+                 **engine_kw) -> Engine:
     """A rollout engine of either family on one GPU; ``engine_kw`` goes to :class:`Engine`."""
     runner, kv = build_runner(cfg, base, num_blocks=num_blocks, block_size=block_size, num_slots=max_num_seqs, device=device,
-                              dtype=dtype, lora_cfg=lora_cfg, max_loras=max_loras)
+                              dtype=dtype, lora_cfg=lora_cfg, max_loras=max_loras, kv_dtype=kv_dtype)
     return Engine(runner, BlockManager(num_blocks, block_size, enable_prefix_caching), eos_token_id=eos_token_id,
                   max_num_seqs=max_num_seqs, max_loras=max_loras, kv_cache=kv, **engine_kw)

@@ -1,5 +1,6 @@
 """Paged KV cache: host-side block accounting (C++ ``csrc/engine/block_manager.cpp``) and the
-per-layer device tensors ``[num_blocks, block_size, Hkv, hd]``.
+per-layer device tensors: bf16 ``[num_blocks, block_size, Hkv, hd]``, or codes of 8 bits with a scale for each block and
+kv head (``ops/kv_q8.py``).
 
 With ``enable_sleep_mode`` the cache can be dropped (``discard``) or copied to pinned host
 memory (``offload`` / ``restore``) while the trainer owns the GPU, mirroring the two sleep
@@ -9,6 +10,7 @@ levels of the reference (``src/art/local/vllm.py:148-231``, ``state.py:146-171``
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -165,8 +167,26 @@ class VmmArena:
             pass
 
 
+#: What ``engine_args.kv_cache_dtype`` may be; the reference passes it to the engine it serves through
+#: (src/art/dev/engine.py:24), whose names these are.  ``int8`` is this package's own.
+KV_CACHE_DTYPES = {"auto": torch.bfloat16, "bfloat16": torch.bfloat16, "fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn,
+                   "int8": torch.int8}
+
+
+def kv_cache_dtype(name: str | torch.dtype | None) -> torch.dtype:
+    """The number format of a cache from its name (None: bf16)."""
+    if isinstance(name, torch.dtype) and name in KV_CACHE_DTYPES.values():
+        return name
+    if name is None or name in KV_CACHE_DTYPES:
+        return KV_CACHE_DTYPES[name or "auto"]
+    raise ValueError(f"kv_cache_dtype {name!r}: supported are {', '.join(KV_CACHE_DTYPES)}")
+
+
 class KVCache:
     """Device tensors of the paged cache, one (k, v) pair per layer.
+
+    ``dtype`` ``torch.float8_e4m3fn`` or ``torch.int8``: codes ``[num_blocks, Hkv, block_size, hd]`` with the scales ``k_scale``
+    and ``v_scale`` ``[num_blocks, Hkv]`` (``ops/kv_q8.py``); ``shape`` names the sizes in the order of the bf16 cache either way.
 
     With ``use_arena`` the tensors live in a :class:`VmmArena`: ``discard`` / ``offload`` hand the physical memory back
     to the driver while every tensor keeps its address, so block tables, captured CUDA graphs and kernel arguments that
@@ -177,33 +197,50 @@ class KVCache:
                  device: torch.device, dtype: torch.dtype = torch.bfloat16, use_arena: bool = False):
         self.shape = (num_blocks, block_size, num_kv_heads, head_dim)
         self.device, self.dtype, self.num_layers = device, dtype, num_layers
-        self.k: list[torch.Tensor] = []
-        self.v: list[torch.Tensor] = []
-        self._host: list[tuple[torch.Tensor, torch.Tensor]] | None = None
+        self.quantised = dtype in (torch.float8_e4m3fn, torch.int8)
+        if self.quantised:
+            from ..ops.kv_q8 import check_geometry
+
+            check_geometry(dtype, block_size, head_dim)
+            part = ((num_blocks, num_kv_heads, block_size, head_dim), dtype)
+            scale = ((num_blocks, num_kv_heads), torch.float32)
+            self._kinds = (part, part, scale, scale)          # of a layer's tensors: k, v and their scales
+        else:
+            self._kinds = ((self.shape, dtype), (self.shape, dtype))
+        self._set([])
+        self._host: list[tuple[torch.Tensor, ...]] | None = None
         self.arena: VmmArena | None = None
-        self._views: tuple[list[torch.Tensor], list[torch.Tensor]] | None = None
+        self._views: list[tuple[torch.Tensor, ...]] | None = None
         if use_arena and torch.device(device).type == "cuda":
-            per = num_blocks * block_size * num_kv_heads * head_dim * torch.empty((), dtype=dtype).element_size()
-            per = (per + 255) // 256 * 256
-            self.arena = VmmArena(2 * num_layers * per, device)
+            sizes = [(math.prod(shape) * t.itemsize + 255) // 256 * 256 for shape, t in self._kinds]
+            self.arena = VmmArena(num_layers * sum(sizes), device)
             self.arena.map()     # views can only be created over mapped memory; they stay valid across unmap / map
-            self._views = ([self.arena.tensor((2 * i) * per, self.shape, dtype) for i in range(num_layers)],
-                           [self.arena.tensor((2 * i + 1) * per, self.shape, dtype) for i in range(num_layers)])
+            at = [sum(sizes[:j]) for j in range(len(sizes))]
+            self._views = [tuple(self.arena.tensor(i * sum(sizes) + at[j], *kind) for j, kind in enumerate(self._kinds))
+                           for i in range(num_layers)]
         self._allocate()
+
+    def _set(self, layers: list[tuple[torch.Tensor, ...]]) -> None:
+        self._layers = layers
+        self.k: list[torch.Tensor] = [t[0] for t in layers]
+        self.v: list[torch.Tensor] = [t[1] for t in layers]
+        self.k_scale: list[torch.Tensor] = [t[2] for t in layers if len(t) > 2]
+        self.v_scale: list[torch.Tensor] = [t[3] for t in layers if len(t) > 2]
 
     def _allocate(self) -> None:
         if self.arena is not None:
             self.arena.map()
-            self.k, self.v = list(self._views[0]), list(self._views[1])
-            for t in self.k + self.v:
-                t.zero_()
+            self._set(list(self._views))
+            for layer in self._layers:
+                for t in layer:
+                    t.zero_()
             return
-        self.k = [torch.zeros(self.shape, dtype=self.dtype, device=self.device) for _ in range(self.num_layers)]
-        self.v = [torch.zeros(self.shape, dtype=self.dtype, device=self.device) for _ in range(self.num_layers)]
+        self._set([tuple(torch.zeros(shape, dtype=t, device=self.device) for shape, t in self._kinds) for _ in range(self.num_layers)])
 
     @staticmethod
     def bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int, head_dim: int, elem: int = 2) -> int:
-        return 2 * num_layers * block_size * num_kv_heads * head_dim * elem
+        """``elem`` 1: a cache in 8 bits, whose blocks have two fp32 scales per kv head beside their codes."""
+        return 2 * num_layers * num_kv_heads * (block_size * head_dim * elem + (4 if elem == 1 else 0))
 
     @property
     def resident(self) -> bool:
@@ -211,7 +248,8 @@ class KVCache:
 
     def discard(self) -> None:
         """Sleep level 2: free the device memory, contents are lost."""
-        self.k, self.v, self._host = [], [], None
+        self._set([])
+        self._host = None
         if self.arena is not None:
             self.arena.unmap()
         elif self.device.type == "cuda":
@@ -220,10 +258,8 @@ class KVCache:
     def offload(self) -> None:
         """Sleep level 1: copy to pinned host memory and free the device memory."""
         pin = self.device.type == "cuda"
-        self._host = [(k.to("cpu", non_blocking=False).pin_memory() if pin else k.clone(),
-                       v.to("cpu", non_blocking=False).pin_memory() if pin else v.clone())
-                      for k, v in zip(self.k, self.v)]
-        self.k, self.v = [], []
+        self._host = [tuple(t.to("cpu", non_blocking=False).pin_memory() if pin else t.clone() for t in layer) for layer in self._layers]
+        self._set([])
         if self.arena is not None:
             self.arena.unmap()
         elif pin:
@@ -237,14 +273,13 @@ class KVCache:
             return
         if self.arena is not None:
             self.arena.map()
-            self.k, self.v = list(self._views[0]), list(self._views[1])
-            for (hk, hv), k, v in zip(self._host, self.k, self.v):
-                k.copy_(hk, non_blocking=True)
-                v.copy_(hv, non_blocking=True)
+            self._set(list(self._views))
+            for host, layer in zip(self._host, self._layers):
+                for h, t in zip(host, layer):
+                    t.copy_(h, non_blocking=True)
             self._host = None
             return
-        self.k = [k.to(self.device, non_blocking=True) for k, _ in self._host]
-        self.v = [v.to(self.device, non_blocking=True) for _, v in self._host]
+        self._set([tuple(t.to(self.device, non_blocking=True) for t in layer) for layer in self._host])
         self._host = None
 
 

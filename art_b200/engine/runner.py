@@ -830,7 +830,9 @@ class NativeRunner(DeviceRunner):
 
         cfg, dev, bs = self.cfg, self.device, self.kv.shape[1]
         Hq, Hkv, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
-        # the rows of attention: every sequence's cached tokens, then its new ones
+        # The rows of attention: every sequence's cached tokens, then its new ones.  A cache in 8 bits gives the tokens of earlier
+        # steps; those of this one are attended to as they were computed, whatever the portions a prompt comes in.
+        from_cache = write_kv and not self.kv.quantised
         tok, pos, slot, held, rows, gid, row_ranges, M, att = [], [], [], [], [], [], [], 0, 0
         for i, s in enumerate(seqs):
             nc, n = s.num_cached, len(s.tokens) if s.upto is None else min(s.upto, len(s.tokens))
@@ -838,9 +840,12 @@ class NativeRunner(DeviceRunner):
             where, in_cache = np.full(len(t), -1), t if write_kv else t[:nc]
             if len(in_cache):
                 where[:len(in_cache)] = np.asarray(s.blocks)[in_cache // bs] * bs + in_cache % bs
+            new_at = where[nc:].copy()
+            if not from_cache:
+                where[nc:] = -1
             tok.append(np.asarray(s.tokens[nc:n], dtype=np.int64))
             pos.append(t[nc:])
-            slot.append(where[nc:] if write_kv else np.full(new, -1))
+            slot.append(new_at if write_kv else np.full(new, -1))
             held.append(where)
             rows.append(att + t[nc:])
             gid.append(np.full(len(t), i))
@@ -873,7 +878,7 @@ class NativeRunner(DeviceRunner):
         def attend(li, fresh=None):
             """Attention of the new tokens, keys and values as the cache holds them.  ``fresh``: the new tokens' queries, and
             their keys and values where the cache does not hold them; None: their queries are in ``buf``."""
-            paged.kv_rows(self.kv.k[li], self.kv.v[li], t_held, buf, cfg.q_size, cfg.q_size + cfg.kv_size)
+            self._read_kv(li, t_held, buf)
             if fresh is not None:
                 buf[:, :fresh.shape[1]].index_copy_(0, t_rows, fresh)
             return new_rows(attn_ops.forward(buf, Hq, Hkv, hd, plan, need_grad=False)[0])
@@ -885,21 +890,30 @@ class NativeRunner(DeviceRunner):
             # few rows: the projections are split and finished as in a decode step
             h, _ = ew.rmsnorm_fwd(x, self.layers[0]["ln1"], cfg.rms_norm_eps, want_rstd=False)
             q = buf[r0:r0 + M, :cfg.q_size] if run else torch.empty((M, cfg.q_size), dtype=buf.dtype, device=dev)
+            kv_rows = self._kv_row_buffers(M)
             for li, L in enumerate(self.layers):
                 def attend_q():
                     if not run:
                         buf[:, :cfg.q_size].index_copy_(0, t_rows, q)
-                    return attend(li)
+                    if not self.kv.quantised:
+                        return attend(li)
+                    if cached:
+                        self._read_kv(li, t_held, buf)
+                    if run:
+                        buf[r0:r0 + M, cfg.q_size:].copy_(kv_rows["kv_rows"])
+                    else:
+                        buf[:, cfg.q_size:].index_copy_(0, t_rows, kv_rows["kv_rows"])
+                    return new_rows(attn_ops.forward(buf, Hq, Hkv, hd, plan, need_grad=False)[0])
                 nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else None
-                x, h = self._layer_fused(li, L, x, h, nxt, t_pos, t_slot, t_ad, any_lora, q, attend_q)
+                x, h = self._layer_fused(li, L, x, h, nxt, t_pos, t_slot, t_ad, any_lora, q, attend_q, kv_rows)
             return x, row_ranges
         whole = not cached and S_att == M       # the projection is the buffer already
         place = not cached and M > 512          # the projection's rows are the buffer's first
         for li, L in enumerate(self.layers):
             qkv = self._qkv(L, x, t_pos, t_ad, any_lora, out=buf[:M] if place else None)
-            paged.kv_write(qkv, cfg.q_size, cfg.q_size + cfg.kv_size, t_slot, self.kv.k[li], self.kv.v[li])
+            self._write_kv(li, qkv, t_slot)
             if cached:
-                o = attend(li, qkv[:, :cfg.q_size if write_kv else buf.shape[1]])
+                o = attend(li, qkv[:, :cfg.q_size if from_cache else buf.shape[1]])
             else:
                 if not (place or whole):
                     buf[:M].copy_(qkv[:, :buf.shape[1]])
@@ -934,7 +948,6 @@ class NativeRunner(DeviceRunner):
         from ..ops import paged
 
         cfg, bs = self.cfg, self.kv.shape[1]
-        Hq, Hkv, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         fused = self._fused_decode_ok(st["tokens"].shape[0])
         for k in range(n_steps):
             x = ew.gather_rows(self.embed, st["tokens"])
@@ -945,14 +958,13 @@ class NativeRunner(DeviceRunner):
                 for li, L in enumerate(self.layers):
                     nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.final_norm
                     x, h = self._layer_fused(li, L, x, h, nxt, st["pos"], st["slot"], st["ad"], any_lora, st["q"],
-                                             lambda: paged.paged_decode_even(st["q"], self.kv.k[li], self.kv.v[li], st["bt"], st["ctx"],
-                                                                             Hq, Hkv, hd, st["attn_out"], st["attn_ws"]))
+                                             lambda: self._attend_cache(li, st["q"], st), st)
                 hidden = h
             else:
                 for li, L in enumerate(self.layers):
                     qkv = self._qkv(L, x, st["pos"], st["ad"], any_lora)
-                    paged.kv_write(qkv, cfg.q_size, cfg.q_size + cfg.kv_size, st["slot"], self.kv.k[li], self.kv.v[li])
-                    paged.paged_decode_even(qkv, self.kv.k[li], self.kv.v[li], st["bt"], st["ctx"], Hq, Hkv, hd, st["attn_out"], st["attn_ws"])
+                    self._write_kv(li, qkv, st["slot"])
+                    self._attend_cache(li, qkv, st)
                     x2 = self._reduce(L["o"](st["attn_out"], st["ad"], any_lora, residual=self._res(x)))
                     x = self._mlp(L, x2, st["ad"], any_lora)
                 hidden, _ = ew.rmsnorm_fwd(x, self.final_norm, cfg.rms_norm_eps, want_rstd=False)
@@ -974,20 +986,67 @@ class NativeRunner(DeviceRunner):
         L = self.layers[0]
         return all(isinstance(L.get(k), EngineLinear) and L[k].cols <= 64 for k in ("qkv", "o", "gu", "down"))
 
-    def _layer_fused(self, li: int, L, x, h, next_norm, pos, slot, adapters, any_lora: bool, q, attend):
+    # -- the cache, in either number format -----------------------------------------------------------
+    def _write_kv(self, li: int, qkv, slot) -> None:
+        """Keys and values of ``qkv`` rows into layer ``li``'s cache."""
+        from ..ops import kv_q8, paged
+
+        kv, k_col = self.kv, self.cfg.q_size
+        if kv.quantised:
+            kv_q8.kv_write_q8(qkv, k_col, k_col + self.cfg.kv_size, slot, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li])
+        else:
+            paged.kv_write(qkv, k_col, k_col + self.cfg.kv_size, slot, kv.k[li], kv.v[li])
+
+    def _read_kv(self, li: int, slot, buf) -> None:
+        """The cached keys and values at ``slot`` into the rows of ``buf``."""
+        from ..ops import kv_q8, paged
+
+        kv, k_col = self.kv, self.cfg.q_size
+        if kv.quantised:
+            kv_q8.kv_rows_q8(kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li], slot, buf, k_col, k_col + self.cfg.kv_size)
+        else:
+            paged.kv_rows(kv.k[li], kv.v[li], slot, buf, k_col, k_col + self.cfg.kv_size)
+
+    def _attend_cache(self, li: int, q, st):
+        """Attention of a decode step's queries over the cache."""
+        from ..ops import kv_q8, paged
+
+        kv, heads = self.kv, (self.cfg.num_heads, self.cfg.num_kv_heads, self.cfg.head_dim)
+        if kv.quantised:
+            return kv_q8.paged_decode_q8(q, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li], st["bt"], st["ctx"], *heads, st["attn_out"],
+                                         st["attn_ws"])
+        return paged.paged_decode_even(q, kv.k[li], kv.v[li], st["bt"], st["ctx"], *heads, st["attn_out"], st["attn_ws"])
+
+    def _kv_row_buffers(self, n: int) -> dict:
+        """Where the keys and values of a few rows are finished before they are quantised: rows [n, k | v] that the finish kernel
+        sees as a cache of 2 n slots, every second of which it writes."""
+        if not self.kv.quantised:
+            return {}
+        return {"kv_rows": torch.zeros((n, 2 * self.cfg.kv_size), dtype=torch.bfloat16, device=self.device),
+                "kv_slot": torch.arange(0, 2 * n, 2, dtype=torch.int32, device=self.device)}
+
+    def _layer_fused(self, li: int, L, x, h, next_norm, pos, slot, adapters, any_lora: bool, q, attend, kv_rows: dict):
         """A layer of a few rows ``x`` whose normed form is ``h``; ``q`` receives the queries, the cache the keys and values,
-        before ``attend()`` gives the attention rows.  Returns the rows after the layer and, with ``next_norm``, their norm."""
-        from ..ops import paged
+        before ``attend()`` gives the attention rows.  ``kv_rows``: :meth:`_kv_row_buffers` of as many rows.  Returns the rows after
+        the layer and, with ``next_norm``, their norm."""
+        from ..ops import kv_q8, paged
 
         cfg = self.cfg
         M, d = x.shape
         ad = adapters if any_lora else None
         lin = L["qkv"]
         w = lin.partial_sums(h, any_lora)
-        paged.decode_finalize_qkv(w, M, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, lin.kpad, pos, cfg.rope_theta, slot,
-                                  self.kv.k[li], self.kv.v[li], q, bias=None if lin.bias_ext is None else lin.bias_ext[:lin.N],
+        kv = self.kv
+        if kv.quantised:
+            rows, at = kv_rows["kv_rows"], kv_rows["kv_slot"]
+            to = (at, rows.view(2 * M, 1, cfg.num_kv_heads, cfg.head_dim), rows[:, cfg.kv_size:])
+        else:
+            to = (slot, kv.k[li], kv.v[li])
+        paged.decode_finalize_qkv(w, M, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, lin.kpad, pos, cfg.rope_theta, *to, q, bias=None if lin.bias_ext is None else lin.bias_ext[:lin.N],
                                   adapter=ad, B_all=lin.B_T, cols=lin.cols, q_norm=L["q_norm"] if cfg.qk_norm else None,
                                   k_norm=L["k_norm"] if cfg.qk_norm else None, eps=cfg.rms_norm_eps)
+        if kv.quantised:
+            kv_q8.kv_write_q8(rows, 0, cfg.kv_size, slot, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li])
         o = attend()
         lin = L["o"]
         w = lin.partial_sums(o, any_lora)
@@ -1013,9 +1072,10 @@ class NativeRunner(DeviceRunner):
         return ew.rmsnorm_fwd(ew.gather_rows(x, rows), self.final_norm, self.cfg.rms_norm_eps, want_rstd=False)[0]
 
     def _decode_buffers(self, nb: int) -> dict:
-        from ..ops import paged
+        from ..ops import kv_q8, paged
 
         cfg = self.cfg
+        workspace = kv_q8.decode_q8_workspace if self.kv.quantised else paged.even_decode_workspace
         return {"attn_out": torch.zeros((nb, cfg.q_size), dtype=torch.bfloat16, device=self.device),
                 "q": torch.zeros((nb, cfg.q_size), dtype=torch.bfloat16, device=self.device),
-                "attn_ws": paged.even_decode_workspace(nb, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, self.device)}
+                "attn_ws": workspace(nb, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, self.device), **self._kv_row_buffers(nb)}

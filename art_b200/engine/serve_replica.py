@@ -24,6 +24,8 @@ import os
 import torch
 import torch.distributed as dist
 
+from .kv_cache import KV_CACHE_DTYPES
+
 
 def build_replica(args):
     from ..local.tokenizer import load_tokenizer
@@ -54,7 +56,7 @@ def build_replica(args):
                 else init_base_weights(cfg, seed=args.seed, dtype=torch.bfloat16, device=dev))
         runner, kv = build_runner(cfg, base, num_blocks=args.num_blocks, block_size=bs, num_slots=args.max_num_seqs, device=dev,
                                   dtype=getattr(torch, args.dtype), lora_cfg=lcfg, max_loras=args.max_loras,
-                                  tp_group=dist.group.WORLD if world > 1 else None)
+                                  tp_group=dist.group.WORLD if world > 1 else None, kv_dtype=args.kv_cache_dtype)
         del base
         torch.cuda.empty_cache()
     tok = load_tokenizer(args.tokenizer or args.weights or f"byte-chat:{args.model}", cfg.vocab_size)
@@ -86,6 +88,7 @@ def main(argv=None) -> None:
     ap.add_argument("--model", default="qwen2.5-7b", help="architecture preset, hybrid presets included (or a name for --weights)")
     ap.add_argument("--weights", default=None, help="directory with config.json and *.safetensors (Hugging Face layout or a hybrid design)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"], help="float32: hybrid models only")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=list(KV_CACHE_DTYPES), help="fp8, int8: twice the tokens in the same memory")
     ap.add_argument("--tokenizer", default=None)
     ap.add_argument("--served-model-name", default=None)
     ap.add_argument("--lora", action="append", help="name=adapter_dir, repeatable")

@@ -100,7 +100,7 @@ class ModelState:
     def __init__(self, base_model: str, config: dev.InternalModelConfig, output_dir: str, rank: int = 0, world: int = 1,
                  tp: int = 1, master_port: int = 0):
         from ..engine.engine import Engine
-        from ..engine.kv_cache import BlockManager
+        from ..engine.kv_cache import BlockManager, kv_cache_dtype
         from ..trainer.trainer import Trainer
 
         init_args = config.get("init_args", {})
@@ -197,13 +197,14 @@ class ModelState:
         # rollout engine: one replica per rank
         block_size = int(engine_args.get("block_size") or 16)
         max_loras = int(engine_args.get("max_loras", 4))
+        kv_dtype = kv_cache_dtype(engine_args.get("kv_cache_dtype"))
         max_len = int(engine_args.get("max_model_len") or init_args.get("max_seq_length", 32768))
         if self.device.type == "cuda":
             from ..engine.factory import build_runner, cache_bytes
 
             free, total = torch.cuda.mem_get_info(self.device)
             util = float(engine_args.get("gpu_memory_utilization", init_args.get("gpu_memory_utilization", 0.5)))
-            per_block, _ = cache_bytes(self.cfg, block_size)
+            per_block, _ = cache_bytes(self.cfg, block_size, kv_dtype=kv_dtype)
             budget = min(free * 0.6, total * util * 0.5)   # leave room for training activations
             num_blocks = int(engine_args.get("num_gpu_blocks_override") or max(64, int(budget // per_block)))
             # sleep mode frees the cache while the trainer runs: the virtual-memory arena keeps every address stable, so
@@ -213,7 +214,7 @@ class ModelState:
             runner, self.kv = build_runner(self.cfg, None if shared else base, num_blocks=num_blocks, block_size=block_size,
                                            device=self.device, lora_cfg=self.lora_cfg, max_loras=max_loras,
                                            decoder=self.trainer.model if shared else None,
-                                           use_arena=bool(engine_args.get("enable_sleep_mode", False)))
+                                           use_arena=bool(engine_args.get("enable_sleep_mode", False)), kv_dtype=kv_dtype)
         else:
             from ..engine.runner import ReferenceRunner
 

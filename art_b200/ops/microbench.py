@@ -389,8 +389,9 @@ def bench_sampler(a) -> dict:
 def bench_paged_decode(a) -> dict:
     """Decode attention over a paged KV cache at a rollout-engine shape: ``seqs`` sequences of ``ctx`` cached tokens,
     ``layers`` distinct caches visited round-robin (together larger than L2, so every launch reads its keys and values
-    from HBM, as in a real step where 28 layers follow one another).  Reports the K+V bytes per second."""
-    from . import _lib, paged
+    from HBM, as in a real step where 28 layers follow one another).  Reports the K+V bytes per second.  ``--cache e4m3 | int8``:
+    a cache in 8 bits (``ops/kv_q8.py``), its bytes."""
+    from . import _lib, kv_q8, paged
 
     dev = "cuda"
     bs = 16
@@ -400,7 +401,15 @@ def bench_paged_decode(a) -> dict:
     for _ in range(a.layers):
         k = (torch.randn(a.seqs * nblk, bs, a.hkv, a.hd, device=dev, generator=g) * 0.5).bfloat16()
         v = (torch.randn(a.seqs * nblk, bs, a.hkv, a.hd, device=dev, generator=g) * 0.5).bfloat16()
-        caches.append((k, v))
+        if a.cache == "bf16":
+            caches.append((k, v))
+            continue
+        n = a.seqs * nblk
+        codes = [torch.zeros(n, a.hkv, bs, a.hd, dtype={"e4m3": torch.float8_e4m3fn, "int8": torch.int8}[a.cache], device=dev) for _ in range(2)]
+        q8 = (*codes, *(torch.zeros(n, a.hkv, device=dev) for _ in range(2)))
+        rows = torch.cat([k.view(n * bs, -1), v.view(n * bs, -1)], 1)
+        kv_q8.kv_write_q8(rows, 0, a.hkv * a.hd, torch.arange(n * bs, dtype=torch.int32, device=dev), *q8)
+        caches.append(q8)
     perm = torch.randperm(a.seqs * nblk, device=dev, generator=g).to(torch.int32)
     width = 64
     while width < nblk:
@@ -413,14 +422,20 @@ def bench_paged_decode(a) -> dict:
     splits = a.splits
     ws = torch.empty(a.seqs * a.hq * splits * (a.hd + 2), dtype=torch.float32, device=dev) if splits > 1 else None
 
+    q8_ws = kv_q8.decode_q8_workspace(a.seqs, a.hq, a.hkv, a.hd, dev) if a.cache != "bf16" else None
+
     def run():                    # one launch per cache, back to back, as the layers of a step follow one another
+        if a.cache != "bf16":
+            for c in caches:
+                kv_q8.paged_decode_q8(q, *c, bt, ctx, a.hq, a.hkv, a.hd, out, q8_ws)
+            return
         for k, v in caches:
             paged.paged_decode(q, k, v, bt, ctx, a.hq, a.hkv, a.hd, out, splits, ws)
 
     ms = _time(run, a.iters, a.warmup, None) / a.layers
     _lib.check_status()
-    kv_bytes = 2.0 * a.seqs * a.ctx * a.hkv * a.hd * 2
-    return {"op": "paged_decode", "seqs": a.seqs, "ctx": a.ctx, "hq": a.hq, "hkv": a.hkv, "hd": a.hd, "splits": splits,
+    kv_bytes = 2.0 * a.seqs * a.ctx * a.hkv * a.hd * (2 if a.cache == "bf16" else 1)
+    return {"op": "paged_decode", "seqs": a.seqs, "ctx": a.ctx, "hq": a.hq, "hkv": a.hkv, "hd": a.hd, "cache": a.cache, "splits": splits,
             "layers": a.layers, "ms": round(ms, 4), "kv_mb": round(kv_bytes / 1e6, 1), "kv_gb_s": round(kv_bytes / ms / 1e6, 1)}
 
 
@@ -482,6 +497,7 @@ def main() -> None:
     pd.add_argument("--hkv", type=int, default=4)
     pd.add_argument("--hd", type=int, default=128)
     pd.add_argument("--splits", type=int, default=1)
+    pd.add_argument("--cache", choices=["bf16", "e4m3", "int8"], default="bf16")
     pd.add_argument("--layers", type=int, default=8, help="distinct caches visited round-robin (8 x 335 MB at the defaults)")
     wg = sub.add_parser("wgrad")
     wg.add_argument("--m", type=int, default=8192)
