@@ -108,9 +108,16 @@ __device__ __forceinline__ uint32_t pq_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void pq_store4(__nv_bfloat16* dst, float a, float b, float c, float d) {
-  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+template <int BYTES>
+__device__ __forceinline__ void pq_put(__nv_bfloat16* dst, const uint32_t* r) {
+  if (BYTES == 8) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(r[0], r[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+  }
 }
+
 template <int N>
 struct PqInt {
   static constexpr int value = N;
@@ -192,8 +199,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   pdl_wait();
   const int Hkv = gridDim.x, kvh = blockIdx.x, shares = gridDim.y, share = blockIdx.y;
   const int table_keys = min(static_cast<long>(max_blocks) * block_size, 0x7fffffffL - PQ_KEYS);
-  auto read_len = [&](int i) {
-    int n = ctx_len[i];
+  auto checked = [&](int n) {
     if (n > table_keys) {
       if (kvh == 0 && share == 0 && status) atomicMax(status, ST_BOUNDS);
       n = table_keys;
@@ -206,19 +212,37 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   // first for themselves, then a scan over the threads.
   const int run = (nseq + PQ_ENTRIES - 1) / PQ_ENTRIES, entries = (nseq + run - 1) / run, mine = (entries + PQ_THREADS - 1) / PQ_THREADS;
   const int e0 = min(entries, tid * mine), e1 = min(entries, e0 + mine);
+  auto empty = [&](int i) {                            // an empty context (the padding of a batch): zeros
+    uint4* o = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * ldo + kvh * G * HD);
+#pragma unroll 1
+    for (int d = 0; d < G * HD / 8; ++d) o[d] = make_uint4(0, 0, 0, 0);
+  };
   int own = 0;
+  if (run == 1) {
+    int len[PQ_ENTRIES / PQ_THREADS];                  // all lengths on their way at once
+#pragma unroll
+    for (int j = 0; j < PQ_ENTRIES / PQ_THREADS; ++j) len[j] = tid + j * PQ_THREADS < nseq ? ctx_len[tid + j * PQ_THREADS] : 0;
+#pragma unroll
+    for (int j = 0; j < PQ_ENTRIES / PQ_THREADS; ++j) {
+      const int i = tid + j * PQ_THREADS;
+      if (i >= nseq) break;
+      const int n = checked(len[j]);
+      s_len[i] = n;
+      if (n == 0 && share == shares - 1) empty(i);
+    }
+    __syncthreads();
+  }
 #pragma unroll 1
   for (int e = e0; e < e1; ++e) {
     s_first[e] = own;
+    if (run == 1) {
+      own += tiles_in(s_len[e]);
+    } else {
 #pragma unroll 1
-    for (int i = e * run; i < min(nseq, (e + 1) * run); ++i) {
-      const int len = read_len(i);
-      s_len[e] = len;                                  // used where run is 1
-      own += tiles_in(len);
-      if (len == 0 && share == shares - 1) {           // an empty context (the padding of a batch): zeros
-        uint4* o = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * ldo + kvh * G * HD);
-#pragma unroll 1
-        for (int d = 0; d < G * HD / 8; ++d) o[d] = make_uint4(0, 0, 0, 0);
+      for (int i = e * run; i < min(nseq, (e + 1) * run); ++i) {
+        const int n = checked(ctx_len[i]);
+        own += tiles_in(n);
+        if (n == 0 && share == shares - 1) empty(i);
       }
     }
   }
@@ -263,11 +287,11 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       int first = s_first[a];
       next.seq = a * run;
-      next.len = run == 1 ? s_len[a] : read_len(next.seq);
+      next.len = run == 1 ? s_len[a] : checked(ctx_len[next.seq]);
 #pragma unroll 1
       while (x >= first + tiles_in(next.len)) {
         first += tiles_in(next.len);
-        next.len = read_len(++next.seq);
+        next.len = checked(ctx_len[++next.seq]);
       }
       next.tile = x - first;
       const int left = next.len - next.tile * PQ_KEYS;
@@ -393,6 +417,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       const int seq = n0.x, tile = n0.y, len = n0.z, keys[2] = {n0.w & 0xff, n0.w >> 8};
       const float ks[2] = {n1.x, n1.y};
       float vs[2] = {n1.z, n1.w};
+      const bool ends = tile + 1 == tiles_in(len);
+      if (ends && i + 1 < tiles) request_q(notes[(i + 1) % PQ_NOTES].seq);
 
       // scores: rows are the keys g and g + 8 of a stretch, columns the heads 2t and 2t + 1
       float s[2][NT][4];
@@ -548,8 +574,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         add(u);
       }
 
-      if (i + 1 == tiles || tile + 1 == tiles_in(len)) {
-        const bool whole = piece_lo == 0 && tile + 1 == tiles_in(len);
+      if (i + 1 == tiles || ends) {
+        const bool whole = piece_lo == 0 && ends;
         // the last piece goes where the tiles were
         float* piece = reinterpret_cast<float*>(i + 1 == tiles ? ring : rings + PQ_WARPS * S::RING + warp * S::PIECE);
         __syncwarp();
@@ -565,9 +591,10 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             if (whole) {
               if (head < G) {
                 __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
+                uint32_t o[JT];
 #pragma unroll
-                for (int j = 0; j < JT; j += 2)
-                  pq_store4(o_row + 2 * j, acc[n][j][x] * f, acc[n][j][2 + x] * f, acc[n][j + 1][x] * f, acc[n][j + 1][2 + x] * f);
+                for (int j = 0; j < JT; ++j) o[j] = pack_bf16x2(acc[n][j][x] * f, acc[n][j][2 + x] * f);
+                pq_put<JT * 4>(o_row, o);
               }
             } else {
               float* dst = piece + head * HD + g * (HD / 8);
@@ -581,7 +608,6 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             }
           }
         if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, lo + i - tile, piece_lo, tile + 1};
-        if (i + 1 < tiles) request_q(notes[(i + 1) % PQ_NOTES].seq);
         piece_lo = 0;                         // the next sequence begins with the next tile
         fresh = true;
       }
@@ -605,11 +631,14 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : pq_exp2(m - top); };
   const int my_seq = lane < 2 * PQ_WARPS ? s_piece[lane].seq : -1;
   uint32_t todo = __ballot_sync(0xffffffffu, my_seq >= 0);
+  bool all_warps = false;                      // one sequence: all warps share its values; several: a warp for each
 #pragma unroll 1
-  while (todo) {
+  for (int k = 0; todo; ++k) {
     const int p0 = __ffs(todo) - 1, seq = __shfl_sync(0xffffffffu, my_seq, p0);
     const uint32_t mine = __ballot_sync(0xffffffffu, my_seq == seq);
     todo &= ~mine;
+    if (k == 0) all_warps = todo == 0;
+    if (!all_warps && k % PQ_WARPS != warp) continue;
     const PqPiece front = s_piece[p0];
     const int hi = s_piece[31 - __clz(mine)].hi, tiles = tiles_in(front.len);
     const bool whole = front.lo == 0 && hi == tiles;
@@ -623,7 +652,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + kvh * G * HD;
     float* to = slot(share, front.lo == 0);
 #pragma unroll 1
-    for (int idx = tid; idx < items; idx += PQ_THREADS) {
+    for (int idx = all_warps ? tid : lane; idx < items; idx += all_warps ? PQ_THREADS : 32) {
       const int r = idx / (HD / 8);
       float m[PQ_WARPS], l[PQ_WARPS], top = -INFINITY;
       PqSum sum{};
@@ -650,7 +679,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
       }
     }
-    if (!whole && tid == 0) {
+    if (!whole && lane == 0 && (!all_warps || warp == 0)) {
       const int sh0 = front.first / per;
       s_part[front.lo == 0] = make_int4(seq, sh0, (front.first + tiles - 1) / per - sh0 + 1, 0);
     }
