@@ -71,4 +71,33 @@ __device__ __forceinline__ void q8_decode4(uint32_t w, float (&f)[4]) {
   }
 }
 
+// What becomes of the scale of a block and head when rows whose largest |value| has the bf16 bits `top` are written to it.
+struct Q8Scale {
+  float to;        // the scale, NaN where a value is not finite: that stays until the block starts anew
+  float inv;       // 1 / to (exact: a power of two), NaN where the codes of the rows are to be zeros
+  float down;      // what the codes of the block's other rows are multiplied by, 1: they stay
+};
+
+// `held`: the scale so far; `anew`: a row at the block's first place is among them.
+template <int KIND>
+__device__ __forceinline__ Q8Scale q8_new_scale(uint32_t top, float held, bool anew) {
+  const float mine = q8_pow2(q8_exponent<KIND>(top < 0x7f80u ? top << 16 : 0u)), none = __int_as_float(0x7fc00000);
+  if (top >= 0x7f80u || (!anew && !(held <= 3.0e38f))) return Q8Scale{none, none, 1.f};
+  const float to = anew ? mine : fmaxf(held, mine), inv = 1.f / to;
+  return Q8Scale{to, inv, !anew && to > held ? held * inv : 1.f};
+}
+
+// 16 codes times `down`, rounded once more; piece v of a block and head.
+template <int KIND>
+__device__ __forceinline__ uint4 q8_lower(uint4 old, float down) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&old);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float f[4];
+    q8_decode4<KIND>(w[j], f);
+    w[j] = q8_encode4<KIND>(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
+  }
+  return old;
+}
+
 }  // namespace artb

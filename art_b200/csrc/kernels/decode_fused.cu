@@ -26,6 +26,7 @@
 
 #include "bounds_check.cuh"
 #include "host_utils.h"
+#include "kv_q8.cuh"
 
 namespace artb {
 
@@ -222,17 +223,66 @@ decode_finalize_norm_kernel(float* __restrict__ ws, int ldw, int N, int kpad, co
 // 512 threads while every row has an SM to itself: the (rope pair | v) units of a row (448 of 32 / 8 heads of 128) are then one
 // pass; 64 such rows with 24 low-rank columns took 19 us in two passes and take 11.  Beyond, two CTAs of 256 threads (128
 // registers) per SM: with 320, which make 28 / 4 heads one pass, registers spill (256 rows: 16 -> 19 us).
-template <int DQ_THREADS>
+//
+// KIND >= 0: the cache is held in 8 bits (kv_q8.cuh), and no two rows of a launch belong to one block.  The lanes that hold a head
+// then agree on its largest value; keys and values are rounded to bf16 first, as the bf16 cache would hold them.  Old scales are
+// read ahead, and blocks whose scale was raised are rounded to it at the end by the whole CTA: one of every ten or so heads of a
+// step is, and eight lanes that did it by themselves held up the launch (6.99 ms a step of 256 sequences of qwen2.5-7b, 6.81 so).
+// Beside a launch of its own for the write: 4.43 ms a step instead of 4.47 (64 sequences of qwen2.5-7b), 6.45 instead of 6.56 (128
+// of qwen3-8b), 6.81 instead of 6.87 (256 of qwen2.5-7b).
+constexpr int DQ_BF16 = -1;
+
+constexpr int DQ_HEADS = 256;        // keys' and values' heads of a cache in 8 bits together
+
+struct Q8Target {
+  float *k_scale, *v_scale;
+  int block_size;
+};
+
+// N values of a head that `width` neighbouring lanes hold, rounded to bf16: 1 / scale of the block that takes them.  `held`: its scale
+// so far, then what the block's other codes are to be multiplied by.
+template <int KIND, int N>
+__device__ __forceinline__ float q8_head_scale(float (&f)[N], float* sp, float* held, bool anew, int width) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t group = ((1u << width) - 1u) << (lane & ~(width - 1));
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    f[e] = __bfloat162float(__float2bfloat16(f[e]));
+    top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+  }
+  for (int o = width >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(group, top, o));
+  const Q8Scale scale = q8_new_scale<KIND>(top >> 16, *held, anew);
+  __syncwarp(group);                   // every lane has the old scale
+  if ((lane & (width - 1)) == 0) {
+    *sp = scale.to;
+    *held = scale.down;
+  }
+  return scale.inv;
+}
+
+template <int KIND>
+__device__ __forceinline__ void q8_store8(uint8_t* dst, const float* f, float inv) {
+  uint2 c = make_uint2(0, 0);
+  if (!isnan(inv)) {
+    c.x = q8_encode4<KIND>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+    c.y = q8_encode4<KIND>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+  }
+  *reinterpret_cast<uint2*>(dst) = c;
+}
+
+template <int DQ_THREADS, int KIND>
 __global__ void __launch_bounds__(DQ_THREADS, DQ_THREADS == 512 ? 1 : 2)
 decode_finalize_qkv_kernel(float* __restrict__ ws, int ldw, int Hq, int Hkv, int hd, int kpad,
                            const float* __restrict__ bias, const int* __restrict__ adapter,
                            const __nv_bfloat16* __restrict__ B_all, int ldb, int cols, const int* __restrict__ pos,
                            float log2_theta, const __nv_bfloat16* __restrict__ q_norm, const __nv_bfloat16* __restrict__ k_norm,
-                           float eps, const int* __restrict__ slot, __nv_bfloat16* __restrict__ k_cache,
-                           __nv_bfloat16* __restrict__ v_cache, __nv_bfloat16* __restrict__ q_out, int ldq,
-                           long num_slots, int* status) {
+                           float eps, const int* __restrict__ slot, void* __restrict__ k_cache_, void* __restrict__ v_cache_,
+                           __nv_bfloat16* __restrict__ q_out, int ldq, long num_slots, int* status, Q8Target q8) {
+  __nv_bfloat16 *k_cache = static_cast<__nv_bfloat16*>(k_cache_), *v_cache = static_cast<__nv_bfloat16*>(v_cache_);
   __shared__ float t_s[DF_MAX_COLS];
   __shared__ float cs_s[128], sn_s[128];     // cos / sin of the row's position for every frequency: shared by all heads
+  __shared__ float held_s[KIND == DQ_BF16 ? 1 : DQ_HEADS];
   warm_expand(adapter, B_all, ldb, cols, (Hq + 2 * Hkv) * hd);
   pdl_wait();                  // attention comes next: its first CTAs would share the few SMs that a product leaves free
   pdl_launch_dependents();
@@ -243,10 +293,18 @@ decode_finalize_qkv_kernel(float* __restrict__ ws, int ldw, int Hq, int Hkv, int
     const float inv_freq = exp2f(-log2_theta * (2.f * threadIdx.x) / hd);
     sincosf(static_cast<float>(pos[row]) * inv_freq, &sn_s[threadIdx.x], &cs_s[threadIdx.x]);
   }
+  int s = slot[row];
+  if (s >= 0 && !(KIND == DQ_BF16 ? index_ok(s, num_slots, status) : q8_index_ok(s, num_slots, status))) s = -1;   // reported, not written
+  const int block = KIND == DQ_BF16 || s < 0 ? 0 : s / q8.block_size, at = KIND == DQ_BF16 || s < 0 ? 0 : s - block * q8.block_size;
+  if constexpr (KIND != DQ_BF16) {
+    if (s >= 0 && static_cast<int>(threadIdx.x) < 2 * Hkv) {
+      const int h = threadIdx.x < Hkv ? threadIdx.x : threadIdx.x - Hkv;
+      held_s[threadIdx.x] = __ldcg((static_cast<int>(threadIdx.x) < Hkv ? q8.k_scale : q8.v_scale) + static_cast<size_t>(block) * Hkv + h);
+    }
+  }
   const int a = stage_shrink(wrow, N, kpad, cols, adapter, row, t_s);      // contains the block barrier
   const __nv_bfloat16* Bs = B_all + (a >= 0 ? static_cast<size_t>(a) * cols * ldb : 0);
-  int s = slot[row];
-  if (s >= 0 && !index_ok(s, num_slots, status)) s = -1;      // checked build: a bad slot is reported, not written
+  auto codes_of = [&](void* cache, int head) { return static_cast<uint8_t*>(cache) + (static_cast<size_t>(block) * Hkv + head) * q8.block_size * hd; };
   const int half = hd >> 1, per_head = half >> 3;
   const int rope_units = (Hq + Hkv) * per_head, v_units = kv_size >> 3;
   for (int u = threadIdx.x; u < rope_units + v_units; u += DQ_THREADS) {
@@ -292,9 +350,22 @@ decode_finalize_qkv_kernel(float* __restrict__ ws, int ldw, int Hq, int Hkv, int
         st8(d, x1);
         st8(d + half, x2);
       } else if (s >= 0) {
-        __nv_bfloat16* d = k_cache + static_cast<size_t>(s) * kv_size + (c1 - q_size);
-        st8(d, x1);
-        st8(d + half, x2);
+        if constexpr (KIND == DQ_BF16) {
+          __nv_bfloat16* d = k_cache + static_cast<size_t>(s) * kv_size + (c1 - q_size);
+          st8(d, x1);
+          st8(d + half, x2);
+        } else {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = x1[e];
+            x[8 + e] = x2[e];
+          }
+          uint8_t* codes = codes_of(k_cache_, h - Hq);
+          const float inv = q8_head_scale<KIND>(x, q8.k_scale + static_cast<size_t>(block) * Hkv + h - Hq, held_s + h - Hq, at == 0, per_head);
+          q8_store8<KIND>(codes + at * hd + vv * 8, x, inv);
+          q8_store8<KIND>(codes + at * hd + half + vv * 8, x + 8, inv);
+        }
       }
     } else {
       const int c = q_size + kv_size + (u - rope_units) * 8;
@@ -302,7 +373,28 @@ decode_finalize_qkv_kernel(float* __restrict__ ws, int ldw, int Hq, int Hkv, int
       take8(wrow + c, x);
       if (bias) add_bias8(x, bias + c);
       if (a >= 0) lora_expand8(x, t_s, Bs, ldb, c, cols);
-      if (s >= 0) st8(v_cache + static_cast<size_t>(s) * kv_size + (c - q_size - kv_size), x);
+      if constexpr (KIND == DQ_BF16) {
+        if (s >= 0) st8(v_cache + static_cast<size_t>(s) * kv_size + (c - q_size - kv_size), x);
+      } else if (s >= 0) {
+        const int h = (u - rope_units) / (2 * per_head), vv = (u - rope_units) - h * 2 * per_head;
+        uint8_t* codes = codes_of(v_cache_, h);
+        const float inv = q8_head_scale<KIND>(x, q8.v_scale + static_cast<size_t>(block) * Hkv + h, held_s + Hkv + h, at == 0, 2 * per_head);
+        q8_store8<KIND>(codes + at * hd + vv * 8, x, inv);
+      }
+    }
+  }
+  if constexpr (KIND != DQ_BF16) {
+    bool raised = false;
+    __syncthreads();
+    if (s >= 0 && static_cast<int>(threadIdx.x) < 2 * Hkv) raised = held_s[threadIdx.x] != 1.f;
+    if (!__syncthreads_or(raised)) return;
+    const int per_row = hd / 16, pieces = q8.block_size * per_row;
+    for (int i = threadIdx.x; i < 2 * Hkv * pieces; i += DQ_THREADS) {
+      const int h = i / pieces, v = i - h * pieces;
+      const float down = held_s[h];
+      if (down == 1.f || v / per_row == at) continue;
+      uint4* p = reinterpret_cast<uint4*>(h < Hkv ? codes_of(k_cache_, h) : codes_of(v_cache_, h - Hkv)) + v;
+      *p = q8_lower<KIND>(*p, down);
     }
   }
 }
@@ -339,11 +431,11 @@ ARTB_EXPORT int artb_decode_finalize_norm(float* ws, int ldw, int M, int N, int 
 
 // q_norm, k_norm (bf16 [hd], or both null): weights of the RMSNorm of each head, hd a power of two.
 // k_cache / v_cache: [slots, Hkv * hd] bf16 (slot = block * block_size + offset; slot[m] < 0: row not written).
-ARTB_EXPORT int artb_decode_finalize_qkv(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int kpad, const float* bias,
-                                         const int* adapter, const void* B_all, int ldb, int cols, const int* pos,
-                                         float theta, const void* q_norm, const void* k_norm, float eps, const int* slot,
-                                         void* k_cache, void* v_cache, void* q_out, int ldq, long num_slots, int* status,
-                                         cudaStream_t st) {
+template <int KIND>
+static int finalize_qkv(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int kpad, const float* bias, const int* adapter,
+                        const void* B_all, int ldb, int cols, const int* pos, float theta, const void* q_norm, const void* k_norm,
+                        float eps, const int* slot, void* k_cache, void* v_cache, void* q_out, int ldq, long num_slots, int* status,
+                        cudaStream_t st, Q8Target q8) {
   if (M <= 0) return 0;
   if ((hd & 15) || hd > 256 || (ldw & 3) || (ldq & 7) || Hq <= 0 || Hkv <= 0 || !pos || !slot) return ERR_BAD_SHAPE;
   if (!q_norm != !k_norm || (q_norm && (hd & (hd - 1)))) return ERR_BAD_SHAPE;
@@ -353,11 +445,38 @@ ARTB_EXPORT int artb_decode_finalize_qkv(float* ws, int ldw, int M, int Hq, int 
     return static_cast<int>(launch_kernel(
         kern, dim3(M), dim3(threads), 0, st, ws, ldw, Hq, Hkv, hd, kpad, bias, adapter,
         reinterpret_cast<const __nv_bfloat16*>(B_all), ldb, cols, pos, log2f(theta),
-        reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps, slot,
-        reinterpret_cast<__nv_bfloat16*>(k_cache), reinterpret_cast<__nv_bfloat16*>(v_cache),
-        reinterpret_cast<__nv_bfloat16*>(q_out), ldq, num_slots, status));
+        reinterpret_cast<const __nv_bfloat16*>(q_norm), reinterpret_cast<const __nv_bfloat16*>(k_norm), eps, slot, k_cache, v_cache,
+        reinterpret_cast<__nv_bfloat16*>(q_out), ldq, num_slots, status, q8));
   };
-  return M <= sm_count() ? go(decode_finalize_qkv_kernel<512>, 512) : go(decode_finalize_qkv_kernel<256>, 256);
+  return M <= sm_count() ? go(decode_finalize_qkv_kernel<512, KIND>, 512) : go(decode_finalize_qkv_kernel<256, KIND>, 256);
+}
+
+ARTB_EXPORT int artb_decode_finalize_qkv(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int kpad, const float* bias,
+                                         const int* adapter, const void* B_all, int ldb, int cols, const int* pos,
+                                         float theta, const void* q_norm, const void* k_norm, float eps, const int* slot,
+                                         void* k_cache, void* v_cache, void* q_out, int ldq, long num_slots, int* status,
+                                         cudaStream_t st) {
+  return finalize_qkv<DQ_BF16>(ws, ldw, M, Hq, Hkv, hd, kpad, bias, adapter, B_all, ldb, cols, pos, theta, q_norm, k_norm, eps, slot,
+                               k_cache, v_cache, q_out, ldq, num_slots, status, st, Q8Target{});
+}
+
+// The same into a cache in 8 bits (codes [num_blocks, Hkv, block_size, hd], scales [num_blocks, Hkv]): no two of the M slots lie in one
+// block.  hd 32, 64 or 128 and an even number of q and k heads together, so that a head's values lie in neighbouring lanes.
+ARTB_EXPORT int artb_decode_finalize_qkv_q8(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int kpad, const float* bias,
+                                            const int* adapter, const void* B_all, int ldb, int cols, const int* pos,
+                                            float theta, const void* q_norm, const void* k_norm, float eps, const int* slot,
+                                            void* k_cache, void* v_cache, float* k_scale, float* v_scale, int block_size, int kind,
+                                            void* q_out, int ldq, long num_blocks, int* status, cudaStream_t st) {
+  if ((hd != 32 && hd != 64 && hd != 128) || ((Hq + Hkv) & 1) || 2 * Hkv > DQ_HEADS || block_size < 16 || (block_size & 15)) return ERR_BAD_SHAPE;
+  const Q8Target q8{k_scale, v_scale, block_size};
+#define ARTB_DQ(KIND_)                                                                                                             \
+  if (kind == KIND_)                                                                                                               \
+  return finalize_qkv<KIND_>(ws, ldw, M, Hq, Hkv, hd, kpad, bias, adapter, B_all, ldb, cols, pos, theta, q_norm, k_norm, eps, slot, \
+                             k_cache, v_cache, q_out, ldq, num_blocks * block_size, status, st, q8)
+  ARTB_DQ(Q8_E4M3);
+  ARTB_DQ(Q8_INT8);
+#undef ARTB_DQ
+  return ERR_BAD_SHAPE;
 }
 
 // Programmatic dependent launch for the kernels of the decode step (see pdl_state in host_utils.h); returns the

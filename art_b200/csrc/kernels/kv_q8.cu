@@ -47,27 +47,22 @@ __device__ __forceinline__ void kw_run(const __nv_bfloat16* x, int ld, int n, in
     }
   }
   top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-
-  const float mine = q8_pow2(q8_exponent<KIND>(top < 0x7f80u ? top << 16 : 0u));
-  const bool anew = at == 0, bad = top >= 0x7f80u || (!anew && !(held <= 3.0e38f));         // not finite
-  const float to = anew ? mine : fmaxf(held, mine), inv = 1.f / to;                         // exact: a power of two
+  const Q8Scale scale = q8_new_scale<KIND>(top, held, at == 0);
+  const float inv = scale.inv;
+  const bool bad = isnan(inv);
   __syncwarp();                              // every lane has the old scale
-  if (lane == 0) *sp = bad ? __int_as_float(0x7fc00000) : to;
-  if (!bad && !anew && to > held) {
-    const float down = held * inv;
-    for (int v = lane; v < block_size * (HD / 16); v += 32) {
-      const int place = v / (HD / 16);
-      if (place >= at && place < at + n) continue;
-      uint4* p = reinterpret_cast<uint4*>(codes) + v;
-      uint4 old = *p;
-      uint32_t* w = reinterpret_cast<uint32_t*>(&old);
+  if (lane == 0) *sp = scale.to;
+  if (scale.down != 1.f) {
+    uint4* p = reinterpret_cast<uint4*>(codes);
+    const int pieces = block_size * (HD / 16);           // four pieces' loads in flight
+    auto other = [&](int v) { return v < pieces && (v / (HD / 16) < at || v / (HD / 16) >= at + n); };
+    for (int v = lane; v < pieces; v += 128) {
+      uint4 old[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f[4];
-        q8_decode4<KIND>(w[j], f);
-        w[j] = q8_encode4<KIND>(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
-      }
-      *p = old;
+      for (int j = 0; j < 4; ++j) old[j] = other(v + 32 * j) ? p[v + 32 * j] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (other(v + 32 * j)) p[v + 32 * j] = q8_lower<KIND>(old[j], scale.down);
     }
   }
   for (int first = 0; first < n; first += BATCH) {

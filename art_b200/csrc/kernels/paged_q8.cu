@@ -22,11 +22,11 @@ namespace artb {
 constexpr int PQ_KEYS = 32;              // keys of a tile: two stretches of 16, each within a block
 constexpr int PQ_WARPS = 4;
 constexpr int PQ_THREADS = PQ_WARPS * 32;
-constexpr int PQ_MIN_TILES = PQ_WARPS;   // tiles of a CTA at least: one per warp
+constexpr int PQ_MIN_TILES = 4;   // tiles of a CTA at least: one per warp
 constexpr int PQ_ENTRIES = 1024;         // of a CTA's list of where sequences begin
 constexpr int PQ_ROUND = 16;             // tiles that a warp looks up at a time
 constexpr int PQ_NOTES = 2 * PQ_ROUND;   // and keeps noted: those in use and the next
-constexpr int PQ_BATCH = 12;             // parts of a sequence that are added up at a time
+constexpr int PQ_BATCH = 4;              // parts of a sequence that are added up at a time
 constexpr float PQ_SLACK = 8.f;          // how far (in powers of two) a score may pass the reference before that moves
 
 __host__ __device__ constexpr int pq_heads(int G) { return G > 8 ? 16 : 8; }
@@ -117,11 +117,6 @@ __device__ __forceinline__ void pq_put(__nv_bfloat16* dst, const uint32_t* r) {
     for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
   }
 }
-
-template <int N>
-struct PqInt {
-  static constexpr int value = N;
-};
 
 // A weighted sum of pieces: eight values of a head, and the sum of its weights.
 struct PqSum {
@@ -697,41 +692,50 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int seq = s_part[k].x, parts = s_part[k].z;
     const size_t stride = static_cast<size_t>(Hkv) * 2 * slot_floats;
     const float* part0 = slot(s_part[k].y, false);           // the first part lies behind it, the others there
-    // parts q0, q0 + 1, ...: their loads in flight together
-    auto add_parts = [&](auto batch, int q0, int idx, PqSum& sum, float& top) {
-      constexpr int N = decltype(batch)::value;
-      const int r = idx / (HD / 8);
-      float m[N], l[N], now = top;
+    constexpr int N = PQ_BATCH;
+    struct Batch {
+      float m[N], l[N];
       float4 a[N], b[N];
+    };
+    // the loads of parts q0, q0 + 1, ... for eight values of head r
+    auto request = [&](Batch& x, int q0, int r, int idx) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        m[j] = -INFINITY;
-        l[j] = 0.f;
-        a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        x.m[j] = -INFINITY;
+        x.l[j] = 0.f;
+        x.a[j] = x.b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (q0 + j < parts) {
           const float* sl = part0 + (q0 + j) * stride + (q0 + j == 0 ? slot_floats : 0);
-          m[j] = __ldcg(sl + G * HD + r);
-          l[j] = __ldcg(sl + G * HD + G + r);
-          a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
-          b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
+          x.m[j] = __ldcg(sl + G * HD + r);
+          x.l[j] = __ldcg(sl + G * HD + G + r);
+          x.a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
+          x.b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
         }
       }
+    };
+    auto add = [&](const Batch& x, PqSum& sum, float& top) {
+      float now = top;
 #pragma unroll
-      for (int j = 0; j < N; ++j) now = fmaxf(now, m[j]);
+      for (int j = 0; j < N; ++j) now = fmaxf(now, x.m[j]);
       sum.scale(top == -INFINITY ? 1.f : pq_exp2(top - now));
       top = now;
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum.add(a[j], b[j], l[j], weight(m[j], l[j], now));
+      for (int j = 0; j < N; ++j) sum.add(x.a[j], x.b[j], x.l[j], weight(x.m[j], x.l[j], now));
     };
 #pragma unroll 1
     for (int idx = tid; idx < items; idx += PQ_THREADS) {
+      const int r = idx / (HD / 8);
       float top = -INFINITY;
       PqSum sum{};
-      if (parts <= 4) {
-        add_parts(PqInt<4>(), 0, idx, sum, top);
-      } else {
+      Batch x, y;
+      request(x, 0, r, idx);
 #pragma unroll 1
-        for (int q0 = 0; q0 < parts; q0 += PQ_BATCH) add_parts(PqInt<PQ_BATCH>(), q0, idx, sum, top);
+      for (int q0 = 0; q0 < parts; q0 += 2 * N) {          // the next batch is on its way while one is added up
+        if (q0 + N < parts) request(y, q0 + N, r, idx);
+        add(x, sum, top);
+        if (q0 + N >= parts) break;
+        if (q0 + 2 * N < parts) request(x, q0 + 2 * N, r, idx);
+        add(y, sum, top);
       }
       sum.store(out + static_cast<size_t>(seq) * ldo + kvh * G * HD + idx * 8);
     }

@@ -958,7 +958,7 @@ class NativeRunner(DeviceRunner):
                 for li, L in enumerate(self.layers):
                     nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.final_norm
                     x, h = self._layer_fused(li, L, x, h, nxt, st["pos"], st["slot"], st["ad"], any_lora, st["q"],
-                                             lambda: self._attend_cache(li, st["q"], st), st)
+                                             lambda: self._attend_cache(li, st["q"], st), st if "kv_rows" in st else {})
                 hidden = h
             else:
                 for li, L in enumerate(self.layers):
@@ -1027,8 +1027,8 @@ class NativeRunner(DeviceRunner):
 
     def _layer_fused(self, li: int, L, x, h, next_norm, pos, slot, adapters, any_lora: bool, q, attend, kv_rows: dict):
         """A layer of a few rows ``x`` whose normed form is ``h``; ``q`` receives the queries, the cache the keys and values,
-        before ``attend()`` gives the attention rows.  ``kv_rows``: :meth:`_kv_row_buffers` of as many rows.  Returns the rows after
-        the layer and, with ``next_norm``, their norm."""
+        before ``attend()`` gives the attention rows.  ``kv_rows``: :meth:`_kv_row_buffers` of as many rows, where several of them may
+        go to one block of a cache in 8 bits.  Returns the rows after the layer and, with ``next_norm``, their norm."""
         from ..ops import kv_q8, paged
 
         cfg = self.cfg
@@ -1036,16 +1036,18 @@ class NativeRunner(DeviceRunner):
         ad = adapters if any_lora else None
         lin = L["qkv"]
         w = lin.partial_sums(h, any_lora)
-        kv = self.kv
-        if kv.quantised:
-            rows, at = kv_rows["kv_rows"], kv_rows["kv_slot"]
-            to = (at, rows.view(2 * M, 1, cfg.num_kv_heads, cfg.head_dim), rows[:, cfg.kv_size:])
-        else:
+        kv, finish = self.kv, paged.decode_finalize_qkv
+        if not kv.quantised:
             to = (slot, kv.k[li], kv.v[li])
-        paged.decode_finalize_qkv(w, M, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, lin.kpad, pos, cfg.rope_theta, *to, q, bias=None if lin.bias_ext is None else lin.bias_ext[:lin.N],
-                                  adapter=ad, B_all=lin.B_T, cols=lin.cols, q_norm=L["q_norm"] if cfg.qk_norm else None,
-                                  k_norm=L["k_norm"] if cfg.qk_norm else None, eps=cfg.rms_norm_eps)
-        if kv.quantised:
+        elif kv_rows:
+            rows = kv_rows["kv_rows"]
+            to = (kv_rows["kv_slot"], rows.view(2 * M, 1, cfg.num_kv_heads, cfg.head_dim), rows[:, cfg.kv_size:])
+        else:
+            finish, to = kv_q8.decode_finalize_qkv_q8, (slot, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li])
+        finish(w, M, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, lin.kpad, pos, cfg.rope_theta, *to, q,
+               bias=None if lin.bias_ext is None else lin.bias_ext[:lin.N], adapter=ad, B_all=lin.B_T, cols=lin.cols,
+               q_norm=L["q_norm"] if cfg.qk_norm else None, k_norm=L["k_norm"] if cfg.qk_norm else None, eps=cfg.rms_norm_eps)
+        if kv.quantised and kv_rows:
             kv_q8.kv_write_q8(rows, 0, cfg.kv_size, slot, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li])
         o = attend()
         lin = L["o"]
@@ -1076,6 +1078,7 @@ class NativeRunner(DeviceRunner):
 
         cfg = self.cfg
         workspace = kv_q8.decode_q8_workspace if self.kv.quantised else paged.even_decode_workspace
+        rows = {} if kv_q8.finalize_covers(cfg.num_heads, cfg.num_kv_heads) else self._kv_row_buffers(nb)
         return {"attn_out": torch.zeros((nb, cfg.q_size), dtype=torch.bfloat16, device=self.device),
                 "q": torch.zeros((nb, cfg.q_size), dtype=torch.bfloat16, device=self.device),
-                "attn_ws": workspace(nb, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, self.device), **self._kv_row_buffers(nb)}
+                "attn_ws": workspace(nb, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, self.device), **rows}

@@ -24,6 +24,8 @@ _sigs = {
     "artb_kv_rows_q8": [vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, ci, cl, ci, vp, vp],
     "artb_paged_decode_q8": [vp, ci, vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, vp, ci, vp, cl, ci, vp, vp],
     "artb_paged_decode_q8_bytes": [ci, ci, ci, ci],
+    "artb_decode_finalize_qkv_q8": [vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, ci, ci, vp, ctypes.c_float, vp, vp, ctypes.c_float, vp, vp,
+                                    vp, vp, vp, ci, ci, vp, ci, cl, vp, vp],
 }
 _bound: dict[str, object] = {}
 
@@ -133,6 +135,35 @@ def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k
     dev = _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
     _launch(dev, "artb_kv_write_q8", qkv.data_ptr(), ld, k_col, v_col, slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, hd, bs, nb, kind)
+
+
+def decode_finalize_qkv_q8(ws: torch.Tensor, M: int, Hq: int, Hkv: int, hd: int, kpad: int, pos: torch.Tensor, theta: float,
+                           slot: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                           v_scale: torch.Tensor, q_out: torch.Tensor, *, bias: torch.Tensor | None = None,
+                           adapter: torch.Tensor | None = None, B_all: torch.Tensor | None = None, cols: int = 0,
+                           q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> None:
+    """:func:`~art_b200.ops.paged.decode_finalize_qkv` into a cache in 8 bits, the same numbers as that and :func:`kv_write_q8` of
+    its bf16 rows in one launch.  No two of the ``M`` slots lie in one block: the rows are those of a decode step.  ``Hq + Hkv`` is
+    even (:func:`finalize_covers`)."""
+    nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
+    if hkv != Hkv or d != hd or not finalize_covers(Hq, Hkv):
+        raise ValueError(f"{Hq} query heads and {Hkv} kv heads of {hd}: the cache has {hkv} of {d}, and the number of both must be even")
+    _index("slot", slot, M)
+    _index("pos", pos, M)
+    n, ldq = _rows("q_out", q_out, 0, 0, Hq * hd)
+    N = (Hq + 2 * Hkv) * hd
+    if ws.dtype is not torch.float32 or ws.dim() != 2 or ws.shape[0] < M or ws.shape[1] < N + (kpad if adapter is not None else 0) or n != M:
+        raise ValueError(f"ws must be fp32 [>= {M}, >= {N} and the low-rank columns], and q_out have {M} rows")
+    dev = _device(ws, pos, slot, k_cache, v_cache, k_scale, v_scale, q_out)
+    ptr = lambda t: 0 if t is None else t.data_ptr()      # noqa: E731
+    _launch(dev, "artb_decode_finalize_qkv_q8", ws.data_ptr(), ws.stride(0), M, Hq, Hkv, hd, kpad, ptr(bias), ptr(adapter), ptr(B_all),
+            B_all.stride(0) if B_all is not None else 0, cols, pos.data_ptr(), theta, ptr(q_norm), ptr(k_norm), eps, slot.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, kind, q_out.data_ptr(), ldq, nb)
+
+
+def finalize_covers(Hq: int, Hkv: int) -> bool:
+    """Whether :func:`decode_finalize_qkv_q8` takes these numbers of heads."""
+    return (Hq + Hkv) % 2 == 0 and Hkv <= 128
 
 
 def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot: torch.Tensor,

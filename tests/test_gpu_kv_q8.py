@@ -373,6 +373,46 @@ def test_graphs_and_streams(dtype):
         assert torch.equal(out, want[0][0]) and torch.equal(x, want[0][1])
 
 
+@KINDS
+@pytest.mark.parametrize("M,Hq,Hkv,hd,bs,lora,norm,bias", [
+    (5, 14, 2, 64, 16, True, False, True),
+    (200, 28, 4, 128, 16, True, False, True),          # two rows to a multiprocessor
+    (33, 32, 8, 128, 48, False, True, False),
+    (1, 3, 1, 32, 16, False, False, True),
+    (64, 4, 2, 32, 32, True, True, False),
+])
+def test_finish_kernel(dtype, M, Hq, Hkv, hd, bs, lora, norm, bias):
+    """The finish kernel into the 8-bit cache: the numbers of the bf16 finish kernel and a write of its rows."""
+    from art_b200.ops import kv_q8, paged
+
+    g = torch.Generator(device=DEV).manual_seed(M + hd)
+    N, kpad, cols, w = (Hq + 2 * Hkv) * hd, 64, 24, Hkv * hd
+    ws = torch.randn(M + 3, N + kpad + 8, generator=g, device=DEV) * torch.exp(0.7 * torch.randn(M + 3, 1, generator=g, device=DEV))
+    kw = dict(bias=torch.randn(N, generator=g, device=DEV) if bias else None, cols=cols,
+              adapter=torch.randint(-1, 2, (M,), generator=g, device=DEV).int() if lora else None,
+              B_all=(0.1 * torch.randn(kpad, N, generator=g, device=DEV)).bfloat16() if lora else None,
+              q_norm=torch.rand(hd, generator=g, device=DEV).bfloat16() if norm else None,
+              k_norm=(torch.rand(hd, generator=g, device=DEV) * 3).bfloat16() if norm else None)
+    pos = torch.randint(0, 5000, (M,), generator=g, device=DEV).int()
+    nb = M + 4
+    block = torch.randperm(nb, generator=g, device=DEV)[:M]
+    slot = (block * bs + torch.randint(0, bs, (M,), generator=g, device=DEV)).int()
+    slot[M // 2] = -1 if M > 1 else slot[0]
+    cache = filled(nb, Hkv, bs, hd, dtype, g)
+    other = [t.clone() for t in cache]
+    args = (M, Hq, Hkv, hd, kpad, pos, 1e6)
+    q1, q2 = (torch.zeros(M, Hq * hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ws1, ws2 = ws.clone(), ws.clone()
+    kv_q8.decode_finalize_qkv_q8(ws1, *args, slot, *cache, q1, **kw)
+    rows = torch.zeros(M, 2 * w, dtype=torch.bfloat16, device=DEV)
+    at = torch.arange(0, 2 * M, 2, dtype=torch.int32, device=DEV)
+    paged.decode_finalize_qkv(ws2, *args, at, rows.view(2 * M, 1, Hkv, hd), rows[:, w:], q2, **kw)
+    kv_q8.kv_write_q8(rows, 0, w, slot, *other)
+    assert torch.equal(q1, q2) and torch.equal(ws1, ws2) and not torch.equal(ws1, ws)
+    for a, b in zip(cache, other):
+        assert torch.equal(a.float(), b.float())
+
+
 def test_places_outside_the_cache_are_reported():
     """Slots, table entries and lengths that name no place are skipped or cut off, and the status word says so."""
     from art_b200.ops import _lib, kv_q8
@@ -395,6 +435,12 @@ def test_places_outside_the_cache_are_reported():
     q = torch.randn(3, Hq * hd, generator=g, device=DEV).bfloat16()
     ws = kv_q8.decode_q8_workspace(3, Hq, Hkv, hd, DEV)
     table = torch.tensor([[0, 1], [2, 3], [4, 5]], dtype=torch.int32, device=DEV)
+    rope = torch.zeros(3, dtype=torch.int32, device=DEV)
+    kv_q8.decode_finalize_qkv_q8(torch.randn(3, (Hq + 2 * Hkv) * hd, generator=g, device=DEV), 3, Hq, Hkv, hd, 0, rope, 1e6, i32(-5, 6 * bs, 2 ** 31 - 1),
+                                 *cache, torch.empty_like(q))
+    with pytest.raises(_lib.KernelStatusError):
+        _lib.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(cache, before))
     good = kv_q8.paged_decode_q8(q, *cache, table, i32(32, 20, 32), Hq, Hkv, hd, torch.empty_like(q), ws)
     _lib.check_status()
     out = kv_q8.paged_decode_q8(q, *cache, table, i32(2 ** 31 - 1, 20, 33), Hq, Hkv, hd, torch.empty_like(q), ws)

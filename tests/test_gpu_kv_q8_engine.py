@@ -96,10 +96,15 @@ def test_portions_attend_to_the_cache_as_it_is(kind, lens, cached):
 
 
 @KINDS
+@pytest.mark.parametrize("finish", [True, False], ids=["finish", "separate"])
 @pytest.mark.parametrize("n,hd,qk_norm", [(5, 128, False), (40, 64, True), (200, 128, False)])
-def test_decode_steps(kind, n, hd, qk_norm):
+def test_decode_steps(kind, n, hd, qk_norm, finish, monkeypatch):
     """A decode step quantises the keys and values it computes into the cache, and its last layer's attention is that of its queries
     over that cache; eager, captured and replayed.  Longer runs draw the tokens that the bf16 engine draws."""
+    from art_b200.ops import kv_q8
+
+    if not finish:       # as with an odd number of heads: rows are finished in bf16 and quantised by a launch of their own
+        monkeypatch.setattr(kv_q8, "finalize_covers", lambda Hq, Hkv: False)
     cfg, base = weights(hd, qk_norm, layers=2)
     lens = [3 + (7 * i) % 60 for i in range(n)]
     q8, kv = runner(cfg, dict(base), kind, blocks=2048)
@@ -122,10 +127,12 @@ def test_decode_steps(kind, n, hd, qk_norm):
         caches = []
         for j, (codes, scale, before) in enumerate(((kv.k[li], kv.k_scale[li], (held[li], held[4 + li])),
                                                      (kv.v[li], kv.v_scale[li], (held[2 + li], held[6 + li])))):
-            o = Cache(*before)
-            o.write(st["kv_rows"][:n, j * w:(j + 1) * w], slots)
-            assert torch.equal(codes.double().cpu(), o.codes) and torch.equal(scale.double().cpu(), o.scale)
-            caches.append(o)
+            now = Cache(codes, scale)
+            if not finish:
+                o = Cache(*before)
+                o.write(st["kv_rows"][:n, j * w:(j + 1) * w], slots)
+                assert torch.equal(now.codes, o.codes) and torch.equal(now.scale, o.scale)
+            caches.append(now)
         for i in range(0, n, max(1, n // 10)):
             at = slots_of(seqs[i], len(seqs[i].tokens))
             ref, bound = attend(st["q"][i].double().cpu().view(cfg.num_heads, hd), caches[0].tokens(at), caches[1].tokens(at))

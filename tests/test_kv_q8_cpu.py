@@ -93,3 +93,26 @@ def test_rows(kw, says):
 def test_decode(kw, says):
     with pytest.raises(ValueError, match=says):
         decode(cache(), **kw)
+
+
+def finish(c, M=3, heads=(4, 2, 64), pos=None, slot=None, q=None, ws=None):
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32)         # noqa: E731
+    kv_q8.decode_finalize_qkv_q8(torch.zeros(4, 512) if ws is None else ws, M, *heads, 0, z(3) if pos is None else pos, 1e6, z(3) if slot is None else slot,
+                                 *c, torch.zeros(3, 256, dtype=BF) if q is None else q)
+
+
+@pytest.mark.parametrize("kw,says", [
+    (dict(heads=(3, 2, 64)), "even"),
+    (dict(heads=(4, 4, 64)), "the cache has 2 of 64"),
+    (dict(heads=(4, 2, 32)), "the cache has 2 of 64"),
+    (dict(M=4), "slot"),
+    (dict(pos=torch.zeros(3)), "pos"),
+    (dict(q=torch.zeros(2, 256, dtype=BF)), "q_out"),
+    (dict(ws=torch.zeros(2, 512)), "ws must be"),
+    (dict(ws=torch.zeros(4, 504)), "ws must be"),
+    (dict(ws=torch.zeros(4, 512, dtype=BF)), "ws must be"),
+    (dict(), "one CUDA device"),
+])
+def test_finish(kw, says):
+    with pytest.raises(ValueError, match=says):
+        finish(cache(), **kw)
