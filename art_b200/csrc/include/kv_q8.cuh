@@ -16,6 +16,26 @@ namespace artb {
 
 enum Q8Kind : int { Q8_E4M3 = 0, Q8_INT8 = 1 };
 
+// Arguments of the launches, as one block of memory each (ops/kv_q8.py packs them).
+struct KvRowsArgs {               // rows [n, ld] bf16 with keys at k_col and values at v_col, their slots, and the cache
+  int* status;
+  void* rows;
+  const int* slot;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  long num_blocks;
+  int n, ld, k_col, v_col, Hkv, hd, block_size, kind;
+};
+struct PagedDecodeArgs {
+  int* status;
+  const void *q, *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int *block_table, *ctx_len;
+  void *out, *ws;
+  long num_blocks;
+  int num_seqs, ldq, ldo, Hq, Hkv, hd, block_size, max_blocks, kind;
+};
+
 constexpr int Q8_LEAST_EXP = -126;       // the smallest scale is a normal fp32 number
 
 // Index checks of these kernels are always on: slots and block tables come from memory, and a compare costs nothing beside

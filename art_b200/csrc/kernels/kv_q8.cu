@@ -20,7 +20,8 @@ namespace artb {
 
 // A run is a stretch of neighbouring rows whose slots are neighbours in one block.  A warp takes a run's part for one kv head, of
 // keys or of values: it looks for the runs that begin among its ROWS rows and follows them to their ends.  A lane holds 8 values
-// of a row, HD / 8 lanes to a row, ITERS * 32 * 8 / HD rows at a time in registers; longer runs are read twice.  FULL: the rows are a multiple of that.
+// of a row, HD / 8 lanes to a row, ITERS * 32 * 8 / HD rows at a time in registers; longer runs are read twice.  FULL: the rows
+// are a multiple of that.
 template <int KIND, int HD, int ITERS, bool FULL>
 __device__ __forceinline__ void kw_run(const __nv_bfloat16* x, int ld, int n, int at, int block_size, uint8_t* codes, float* sp) {
   constexpr int LPR = HD / 8, RPI = 32 / LPR, BATCH = ITERS * RPI;
@@ -53,16 +54,10 @@ __device__ __forceinline__ void kw_run(const __nv_bfloat16* x, int ld, int n, in
   __syncwarp();                              // every lane has the old scale
   if (lane == 0) *sp = scale.to;
   if (scale.down != 1.f) {
-    uint4* p = reinterpret_cast<uint4*>(codes);
-    const int pieces = block_size * (HD / 16);           // four pieces' loads in flight
-    auto other = [&](int v) { return v < pieces && (v / (HD / 16) < at || v / (HD / 16) >= at + n); };
-    for (int v = lane; v < pieces; v += 128) {
-      uint4 old[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) old[j] = other(v + 32 * j) ? p[v + 32 * j] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (other(v + 32 * j)) p[v + 32 * j] = q8_lower<KIND>(old[j], scale.down);
+    for (int v = lane; v < block_size * (HD / 16); v += 32) {
+      if (v / (HD / 16) >= at && v / (HD / 16) < at + n) continue;
+      uint4* p = reinterpret_cast<uint4*>(codes) + v;
+      *p = q8_lower<KIND>(*p, scale.down);
     }
   }
   for (int first = 0; first < n; first += BATCH) {
@@ -196,21 +191,21 @@ kv_rows_q8_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
 
 using namespace artb;
 
-// qkv [M, ld] bf16 with keys at k_col and values at v_col; slot [M]: block * block_size + place, < 0: the row is not written.
+// slot: block * block_size + place, < 0: the row is not written.
 // A slot beyond the cache is not written either and reported through `status`.
-ARTB_EXPORT int artb_kv_write_q8(const void* qkv, int ld, int k_col, int v_col, const int* slot, void* k_cache, void* v_cache,
-                                 float* k_scale, float* v_scale, int M, int Hkv, int hd, int block_size, long num_blocks,
-                                 int kind, int* status, cudaStream_t st) {
+ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
+  const int M = a->n, ld = a->ld, Hkv = a->Hkv, hd = a->hd, block_size = a->block_size, kind = a->kind;
   if (M <= 0) return 0;
-  if (Hkv <= 0 || block_size < 16 || (block_size & 15) || (ld & 7) || (k_col & 7) || (v_col & 7)) return ERR_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return ERR_BAD_ALIGN;
+  if (Hkv <= 0 || block_size < 16 || (block_size & 15) || (ld & 7) || (a->k_col & 7) || (a->v_col & 7)) return ERR_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->rows) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) return ERR_BAD_ALIGN;
   const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
 #define ARTB_KW(KIND_, HD_)                                                                                                  \
   if (kind == KIND_ && hd == HD_) {                                                                                          \
     auto go = [&](auto kern, int rows) {                                                                                     \
       return static_cast<int>(launch_kernel(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), 0, st,          \
-                                            (const __nv_bfloat16*)qkv, ld, k_col, v_col, slot, (uint8_t*)k_cache,            \
-                                            (uint8_t*)v_cache, k_scale, v_scale, M, Hkv, block_size, shift, num_blocks, status)); \
+                                            (const __nv_bfloat16*)a->rows, ld, a->k_col, a->v_col, a->slot,                  \
+                                            (uint8_t*)a->k_cache, (uint8_t*)a->v_cache, a->k_scale, a->v_scale, M, Hkv,      \
+                                            block_size, shift, a->num_blocks, a->status));                                   \
     };                                                                                                                       \
     if (M <= 256) return go(kv_write_q8_kernel<KIND_, HD_, 1>, 1);                                                           \
     if (M <= 2048) return go(kv_write_q8_kernel<KIND_, HD_, 4>, 4);                                                          \
@@ -222,21 +217,20 @@ ARTB_EXPORT int artb_kv_write_q8(const void* qkv, int ld, int k_col, int v_col, 
   return ERR_BAD_SHAPE;
 }
 
-ARTB_EXPORT int artb_kv_rows_q8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
-                                const int* slot, int n, void* dst, int ld, int k_col, int v_col, int Hkv, int hd, int block_size,
-                                long num_blocks, int kind, int* status, cudaStream_t st) {
+ARTB_EXPORT int artb_kv_rows_q8(const KvRowsArgs* a, cudaStream_t st) {
+  const int n = a->n, ld = a->ld, Hkv = a->Hkv, hd = a->hd, block_size = a->block_size, kind = a->kind;
   if (n <= 0) return 0;
-  if (Hkv <= 0 || hd < 16 || (hd & 15) || block_size < 1 || (ld & 7) || (k_col & 7) || (v_col & 7)) return ERR_BAD_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) return ERR_BAD_ALIGN;
+  if (Hkv <= 0 || hd < 16 || (hd & 15) || block_size < 1 || (ld & 7) || (a->k_col & 7) || (a->v_col & 7)) return ERR_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->rows) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) return ERR_BAD_ALIGN;
   const int vec = Hkv * hd / 8, bx = vec < 256 ? vec : 256, by = 256 / bx;
   const bool once = (static_cast<long>(n) + by - 1) / by <= 8L * sm_count();
   const long blocks = (static_cast<long>(n) + by * (once ? 1 : 4) - 1) / (by * (once ? 1 : 4));
   const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
-  const bool wide = ((reinterpret_cast<uintptr_t>(dst) & 31) | (ld & 15) | (k_col & 15) | (v_col & 15)) == 0;
+  const bool wide = ((reinterpret_cast<uintptr_t>(a->rows) & 31) | (ld & 15) | (a->k_col & 15) | (a->v_col & 15)) == 0;
   auto go = [&](auto kern) {
     kern<<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), dim3(bx, by), 0, st>>>(
-        (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, slot, n, (__nv_bfloat16*)dst, ld, k_col, v_col, Hkv, hd,
-        block_size, shift, num_blocks, status);
+        (const uint8_t*)a->k_cache, (const uint8_t*)a->v_cache, a->k_scale, a->v_scale, a->slot, n, (__nv_bfloat16*)a->rows, ld,
+        a->k_col, a->v_col, Hkv, hd, block_size, shift, a->num_blocks, a->status);
     return (int)cudaGetLastError();
   };
 #define ARTB_KR(KIND_)                                                                                                     \

@@ -778,10 +778,9 @@ ARTB_EXPORT int artb_paged_decode_q8_bytes(int num_seqs, int Hq, int Hkv, int hd
 
 // q [num_seqs, ldq], out [num_seqs, ldo] bf16; block_table [num_seqs, max_blocks]; a context that its table row cannot hold is cut
 // off, keys whose table entry is no block are left out, and both are reported through `status`.
-ARTB_EXPORT int artb_paged_decode_q8(const void* q, int ldq, const void* k_cache, const void* v_cache, const float* k_scale,
-                                     const float* v_scale, const int* block_table, int max_blocks, const int* ctx_len,
-                                     int block_size, int num_seqs, int Hq, int Hkv, int hd, void* out, int ldo, void* ws,
-                                     long num_blocks, int kind, int* status, cudaStream_t st) {
+ARTB_EXPORT int artb_paged_decode_q8(const PagedDecodeArgs* args, cudaStream_t st) {
+  const auto [status, q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws, num_blocks, num_seqs, ldq, ldo, Hq, Hkv, hd,
+              block_size, max_blocks, kind] = *args;
   if (num_seqs <= 0) return 0;
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 16 || block_size < 16 || (block_size & 15) || max_blocks < 1 || num_blocks < 1 || (ldq & 7) ||
       (ldo & 7) || !ws)

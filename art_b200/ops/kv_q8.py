@@ -13,16 +13,22 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 
 import torch
 
 from . import _lib
 
 vp, ci, cl = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+# The launches that a layer makes take their arguments as one block of memory, laid out as the C structs of these names
+# (csrc/include/kv_q8.cuh): ctypes takes 0.1 us for each argument that it converts, and the kernels take a few.
+_blocks = {
+    "artb_kv_write_q8": struct.Struct("PPPPPPP q iiiiiiii"),
+    "artb_kv_rows_q8": struct.Struct("PPPPPPP q iiiiiiii"),
+    "artb_paged_decode_q8": struct.Struct("PPPPPPPPPP q iiiiiiiii"),
+}
 _sigs = {
-    "artb_kv_write_q8": [vp, ci, ci, ci, vp, vp, vp, vp, vp, ci, ci, ci, ci, cl, ci, vp, vp],
-    "artb_kv_rows_q8": [vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, ci, cl, ci, vp, vp],
-    "artb_paged_decode_q8": [vp, ci, vp, vp, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, vp, ci, vp, cl, ci, vp, vp],
+    **{name: [ctypes.c_char_p, vp] for name in _blocks},
     "artb_paged_decode_q8_bytes": [ci, ci, ci, ci],
     "artb_decode_finalize_qkv_q8": [vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, ci, ci, vp, ctypes.c_float, vp, vp, ctypes.c_float, vp, vp,
                                     vp, vp, vp, ci, ci, vp, ci, cl, vp, vp],
@@ -102,19 +108,23 @@ def _index(name: str, t: torch.Tensor, n: int) -> None:
 
 def _device(*tensors: torch.Tensor) -> int:
     """Number of the CUDA device that all tensors lie on."""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != dev or dev < 0:
-            raise ValueError(f"tensors of one CUDA device are needed: {', '.join(sorted({str(t.device) for t in tensors}))}")
+    devices = {t.get_device() for t in tensors}
+    dev = devices.pop()
+    if devices or dev < 0:
+        raise ValueError(f"tensors of one CUDA device are needed: {', '.join(sorted({str(t.device) for t in tensors}))}")
     return dev
 
 
 def _launch(dev: int, name: str, *args) -> None:
-    """On the current stream of device ``dev``, whichever device is current."""
+    """On the current stream of device ``dev``, whichever device is current; ``args`` end before the status word."""
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _launch(dev, name, *args)
-    rc = _f(name)(*args, _lib.status_word(dev).data_ptr(), _lib.raw_stream(dev))
+    fn, block, word = _bound.get(name) or _f(name), _blocks.get(name), _lib.status_word(dev).data_ptr()
+    if block is not None:
+        rc = fn(block.pack(word, *args), _lib.raw_stream(dev))
+    else:
+        rc = fn(*args, word, _lib.raw_stream(dev))
     if rc:
         _lib.check_rc(rc, name.removeprefix("artb_"))
     _lib.LAUNCHES += 1
@@ -133,8 +143,8 @@ def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k
     n, ld = _rows("qkv", qkv, k_col, v_col, hkv * hd)
     _index("slot", slot, n)
     dev = _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_write_q8", qkv.data_ptr(), ld, k_col, v_col, slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, hd, bs, nb, kind)
+    _launch(dev, "artb_kv_write_q8", qkv.data_ptr(), slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), nb, n, ld, k_col, v_col, hkv, hd, bs, kind)
 
 
 def decode_finalize_qkv_q8(ws: torch.Tensor, M: int, Hq: int, Hkv: int, hd: int, kpad: int, pos: torch.Tensor, theta: float,
@@ -178,8 +188,8 @@ def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     if n > have:
         raise ValueError(f"{n} slots for {have} rows")
     dev = _device(dst, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_rows_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slot.data_ptr(), n,
-            dst.data_ptr(), ld, k_col, v_col, hkv, hd, bs, nb, kind)
+    _launch(dev, "artb_kv_rows_q8", dst.data_ptr(), slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), nb, n, ld, k_col, v_col, hkv, hd, bs, kind)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -214,6 +224,6 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     dev = _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
     if n and (ws.nbytes < _decode_bytes(n, Hq, Hkv, hd, dev) or not ws.is_contiguous()):
         raise ValueError(f"workspace of {ws.nbytes} bytes, {_decode_bytes(n, Hq, Hkv, hd, dev)} needed in a row")
-    _launch(dev, "artb_paged_decode_q8", q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            block_table.data_ptr(), table[1], ctx_len.data_ptr(), bs, n, Hq, Hkv, hd, out.data_ptr(), ldo, ws.data_ptr(), nb, kind)
+    _launch(dev, "artb_paged_decode_q8", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), ctx_len.data_ptr(), out.data_ptr(), ws.data_ptr(), nb, n, ldq, ldo, Hq, Hkv, hd, bs, table[1], kind)
     return out
