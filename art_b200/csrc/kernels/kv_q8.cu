@@ -104,7 +104,10 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
   const int blk = s < 0 ? 0 : block_shift >= 0 ? s >> block_shift : s / block_size;
   const bool goes_on = s > 0 && prev == s - 1 && s != blk * block_size;        // with the run of the row before
   const uint32_t on = __ballot_sync(0xffffffffu, goes_on);
-  for (uint32_t todo = __ballot_sync(0xffffffffu, lane < ROWS && s >= 0 && !goes_on); todo; todo &= todo - 1) {
+  // a second run in the block of the row before would be a second warp's at the same scale: refused
+  const bool astray = s >= 0 && !goes_on && prev >= blk * block_size && prev - blk * block_size < block_size;
+  if (astray && lane < ROWS && status) atomicMax(status, ST_BAD_ARGS);
+  for (uint32_t todo = __ballot_sync(0xffffffffu, lane < ROWS && s >= 0 && !goes_on && !astray); todo; todo &= todo - 1) {
     const int i = __ffs(todo) - 1, s0 = __shfl_sync(0xffffffffu, s, i), block = __shfl_sync(0xffffffffu, blk, i);
     if (!q8_index_ok(s0, num_blocks * block_size, status)) continue;
     const int r0 = row0 + i, at = s0 - block * block_size;

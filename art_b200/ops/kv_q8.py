@@ -133,8 +133,9 @@ def _launch(dev: int, name: str, *args) -> None:
 def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
     """Quantises the keys and values of the rows of ``qkv`` (bf16 [M, >= ...], columns ``k_col`` and ``v_col`` on) into the cache.
-    ``slot`` int32 [M]: block * block_size + place, negative: the row is not written.  The rows of a block stand next to each other
-    in the order of their places, and a slot occurs once.
+    ``slot`` int32 [M]: block * block_size + place, negative: the row is not written.  The rows that go to one block are neighbours and
+    go to consecutive places, as those of a prompt and of a decode step do; a row that follows one of its block elsewhere is not
+    written and reported through the status word, as are slots beyond the cache.
 
     The scale of a block and head is the least power of two that takes the largest value written to it into the range of the
     codes.  A row at a block's first place starts the block anew.  Rows at later places can only raise the scale, and then what
@@ -199,7 +200,7 @@ def _decode_bytes(n: int, Hq: int, Hkv: int, hd: int, device: int) -> int:
 
 
 def decode_q8_workspace(n: int, Hq: int, Hkv: int, hd: int, device) -> torch.Tensor:
-    """Workspace of :func:`paged_decode_q8` for up to ``n`` sequences; one call at a time may use it."""
+    """Workspace of :func:`paged_decode_q8` for up to ``n`` sequences of these heads; one call at a time may use it."""
     dev = torch.device(device)
     index = torch.cuda.current_device() if dev.index is None else dev.index
     return torch.zeros(_decode_bytes(n, Hq, Hkv, hd, index), dtype=torch.uint8, device=dev)
@@ -209,14 +210,16 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     block_table: torch.Tensor, ctx_len: torch.Tensor, Hq: int, Hkv: int, hd: int, out: torch.Tensor,
                     ws: torch.Tensor) -> torch.Tensor:
     """Attention of one token per sequence over the first ``ctx_len`` cached tokens: q bf16 [n, >= Hq*hd] (row stride arbitrary),
-    ``block_table`` int32 [n, width], ``ctx_len`` int32 [n] (0: the row becomes zeros); out bf16 [n, >= Hq*hd]."""
+    ``block_table`` int32 [n, width], ``ctx_len`` int32 [n] (0: the row becomes zeros); out bf16 [n, >= Hq*hd].  Scales are as
+    :func:`kv_write_q8` leaves them.  Entries that are no block and lengths that the table cannot hold are reported through the
+    status word; such keys are left out.  The same inputs give the same bits."""
     nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
     if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > 16 * Hkv:
         raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
     n, ldq = _rows("q", q, 0, 0, Hq * hd)
     m, ldo = _rows("out", out, 0, 0, Hq * hd)
-    if m != n or ldo < Hq * hd:
-        raise ValueError(f"out must have {n} rows that do not overlap")
+    if m != n or ldo < Hq * hd or (n and out.data_ptr() == q.data_ptr()):
+        raise ValueError(f"out must have {n} rows that do not overlap, nor lie where q does")
     _index("ctx_len", ctx_len, n)
     table = block_table.shape
     if block_table.dtype is not torch.int32 or len(table) != 2 or table[0] != n or table[1] < 1 or not block_table.is_contiguous():

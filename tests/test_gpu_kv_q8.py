@@ -209,6 +209,11 @@ DECODE = [
     ([1500] * 64, 8, 8, 64, 32),
     ([19, 4001], 9, 1, 128, 128),
     ([0, 0, 0], 4, 2, 32, 16),
+    ([(5 * i) % 70 for i in range(1500)], 4, 2, 64, 16),          # more sequences than a CTA lists one by one
+    ([0] * 2000 + [40, 0, 300] + [0] * 1500 + [1], 4, 1, 128, 16),
+    ([3] * 1024, 4, 4, 32, 16),
+    ([90] * 40, 128, 64, 64, 16),                                 # many kv heads
+    ([70, 900], 600, 600, 32, 16),                                # more than CTAs
     ([300, 0, 0, 0, 0, 2, 0, 64], 6, 2, 128, 64),
 ]
 
@@ -452,6 +457,24 @@ def test_places_outside_the_cache_are_reported():
     with pytest.raises(_lib.KernelStatusError):
         _lib.check_status()
     assert torch.equal(out[1], good[1]) and out.isfinite().all()
+
+
+def test_rows_of_a_block_that_are_not_in_order_are_refused():
+    """A row after another of its block that is not at the next place: not written, and the status word says so."""
+    from art_b200.ops import _lib, kv_q8
+
+    Hkv, hd, bs = 2, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(8)
+    for slots, written in (([5, 7], [5, -1]), ([5, 5], [5, -1]), ([5, 4], [5, -1]), ([3, 4, 20, 22, 21], [3, 4, 20, -1, -1])):
+        cache = filled(3, Hkv, bs, hd, E4, g)
+        o = oracles_of(cache)
+        x = keys(len(slots), Hkv, hd, g)
+        kv_q8.kv_write_q8(x, 0, Hkv * hd, torch.tensor(slots, dtype=torch.int32, device=DEV), *cache)
+        with pytest.raises(_lib.KernelStatusError):
+            _lib.check_status()
+        for j in range(2):
+            o[j].write(x[:, j * Hkv * hd:(j + 1) * Hkv * hd], written)
+        same(cache, *o)
 
 
 def test_caches_beyond_32_bits():

@@ -22,6 +22,9 @@ def rows(c, dst=None, slot=None, k_col=0, v_col=128):
     kv_q8.kv_rows_q8(*c, torch.zeros(3, dtype=torch.int32) if slot is None else slot, dst, k_col, v_col)
 
 
+SAME = torch.zeros(3, 256, dtype=BF)
+
+
 def decode(c, q=None, table=None, ctx=None, heads=(4, 2, 64), out=None, ws=None):
     z = lambda *s: torch.zeros(*s, dtype=torch.int32)         # noqa: E731
     q = torch.zeros(3, 256, dtype=BF) if q is None else q
@@ -83,6 +86,7 @@ def test_rows(kw, says):
     (dict(q=torch.zeros(3, 256)), "bf16"),
     (dict(out=torch.zeros(2, 256, dtype=BF)), "out must have 3 rows"),
     (dict(out=torch.zeros(1, 256, dtype=BF).expand(3, 256)), "overlap"),
+    (dict(q=SAME, out=SAME), "nor lie where q does"),
     (dict(table=torch.zeros(2, 2, dtype=torch.int32)), "block_table"),
     (dict(table=torch.zeros(3, 0, dtype=torch.int32)), "block_table"),
     (dict(table=torch.zeros(3, 2)), "block_table"),
