@@ -113,6 +113,14 @@ inline cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, 
   return launch_ordered(pdl_state().mode != 0, kern, grid, block, smem, stream, static_cast<Args&&>(args)...);
 }
 
+// Kernels without tensor memory whose first access to global memory is behind pdl_wait(), their own arguments aside: they may start
+// ahead of what comes before them whatever that is, switch or no switch, and what comes after them keeps its own order.  About
+// 2 us of a launch between others.
+template <class... KArgs, class... Args>
+inline cudaError_t launch_ahead(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+  return launch_ordered(true, kern, grid, block, smem, stream, static_cast<Args&&>(args)...);
+}
+
 // products with tiles of CTAS CTAs
 template <int CTAS, class... KArgs, class... Args>
 inline cudaError_t launch_product(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {

@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(256)
 kv_rows_q8_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const float* __restrict__ k_scale,
                   const float* __restrict__ v_scale, const int* __restrict__ slot, int n, __nv_bfloat16* __restrict__ dst, int ld,
                   int k_col, int v_col, int Hkv, int hd, int block_size, int block_shift, long num_blocks, int* status) {
+  pdl_wait();
+  pdl_launch_dependents();
   const int half = Hkv * hd / 16;
   for (int at = threadIdx.x; at < 2 * half; at += blockDim.x) {
     const bool is_v = at >= half;
@@ -205,7 +207,7 @@ ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
 #define ARTB_KW(KIND_, HD_)                                                                                                  \
   if (kind == KIND_ && hd == HD_) {                                                                                          \
     auto go = [&](auto kern, int rows) {                                                                                     \
-      return static_cast<int>(launch_kernel(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), 0, st,          \
+      return static_cast<int>(launch_ahead(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), 0, st,          \
                                             (const __nv_bfloat16*)a->rows, ld, a->k_col, a->v_col, a->slot,                  \
                                             (uint8_t*)a->k_cache, (uint8_t*)a->v_cache, a->k_scale, a->v_scale, M, Hkv,      \
                                             block_size, shift, a->num_blocks, a->status));                                   \
@@ -231,10 +233,10 @@ ARTB_EXPORT int artb_kv_rows_q8(const KvRowsArgs* a, cudaStream_t st) {
   const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
   const bool wide = ((reinterpret_cast<uintptr_t>(a->rows) & 31) | (ld & 15) | (a->k_col & 15) | (a->v_col & 15)) == 0;
   auto go = [&](auto kern) {
-    kern<<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), dim3(bx, by), 0, st>>>(
-        (const uint8_t*)a->k_cache, (const uint8_t*)a->v_cache, a->k_scale, a->v_scale, a->slot, n, (__nv_bfloat16*)a->rows, ld,
-        a->k_col, a->v_col, Hkv, hd, block_size, shift, a->num_blocks, a->status);
-    return (int)cudaGetLastError();
+    return static_cast<int>(launch_ahead(kern, dim3(static_cast<unsigned>(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(bx, by), 0, st,
+                                         (const uint8_t*)a->k_cache, (const uint8_t*)a->v_cache, a->k_scale, a->v_scale, a->slot, n,
+                                         (__nv_bfloat16*)a->rows, ld, a->k_col, a->v_col, Hkv, hd, block_size, shift, a->num_blocks,
+                                         a->status));
   };
 #define ARTB_KR(KIND_)                                                                                                     \
   if (kind == KIND_) {                                                                                                     \

@@ -812,7 +812,7 @@ ARTB_EXPORT int artb_paged_decode_q8(const PagedDecodeArgs* args, cudaStream_t s
       if (e != cudaSuccess) return static_cast<int>(e);                                                                       \
       cfgd[dev_] = true;                                                                                                      \
     }                                                                                                                         \
-    return static_cast<int>(launch_kernel(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(Hkv, shares), dim3(PQ_THREADS),       \
+    return static_cast<int>(launch_ahead(paged_decode_q8_kernel<KIND_, HD_, HEADS_>, dim3(Hkv, shares), dim3(PQ_THREADS),       \
                                           PqSmem<HD_, HEADS_>::BYTES, st, k_map, v_map, (const __nv_bfloat16*)q, ldq,         \
                                           k_scale, v_scale, block_table, max_blocks, ctx_len, block_size, sub_shift, num_seqs, \
                                           Hq / Hkv, per_share, (__nv_bfloat16*)out, ldo, part, count, scale_log2, num_blocks, \
