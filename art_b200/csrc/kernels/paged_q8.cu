@@ -622,8 +622,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const int slot_floats = pq_piece_floats(G, HD), items = G * (HD / 8);           // a thread adds up 8 values of a head
   // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
   auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
-  // what holds nothing has no reference, or has met a value that is not a number
-  auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : pq_exp2(m - top); };
+  // of a piece with reference m beside the largest of them, which is -inf where none has one; sums that are not numbers stay so
+  auto weight = [](float m, float top) { return pq_exp2(m - (top == -INFINITY ? 0.f : top)); };
   const int my_seq = lane < 2 * PQ_WARPS ? s_piece[lane].seq : -1;
   uint32_t todo = __ballot_sync(0xffffffffu, my_seq >= 0);
   bool all_warps = false;                      // one sequence: all warps share its values; several: a warp for each
@@ -661,7 +661,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       for (int w = 0; w < PQ_WARPS; ++w)
         if (from[w]) {
           const float4* v = reinterpret_cast<const float4*>(from[w]) + idx * 2;
-          sum.add(v[0], v[1], l[w], weight(m[w], l[w], top));
+          sum.add(v[0], v[1], l[w], weight(m[w], top));
         }
       if (whole) {
         sum.store(o_row + idx * 8);
@@ -681,9 +681,9 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   __syncthreads();
   if (warp < 2 && lane == 0 && s_part[warp].z > 0) {
-    __threadfence();                                         // of what the CTA wrote before the barrier
-    s_part[warp].w = atomicAdd(&count[s_part[warp].x * Hkv + kvh], 1) == s_part[warp].z - 1;
-    __threadfence();
+    int seen;                                                // releases what the CTA wrote before the barrier
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(&count[s_part[warp].x * Hkv + kvh]) : "memory");
+    s_part[warp].w = seen == s_part[warp].z - 1;
   }
   __syncthreads();
 #pragma unroll 1
@@ -717,10 +717,10 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       float now = top;
 #pragma unroll
       for (int j = 0; j < N; ++j) now = fmaxf(now, x.m[j]);
-      sum.scale(top == -INFINITY ? 1.f : pq_exp2(top - now));
+      sum.scale(weight(top, now));
       top = now;
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum.add(x.a[j], x.b[j], x.l[j], weight(x.m[j], x.l[j], now));
+      for (int j = 0; j < N; ++j) sum.add(x.a[j], x.b[j], x.l[j], weight(x.m[j], now));
     };
 #pragma unroll 1
     for (int idx = tid; idx < items; idx += PQ_THREADS) {

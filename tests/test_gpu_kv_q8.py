@@ -284,6 +284,30 @@ def test_decode_keeps_what_is_masked_out():
 
 
 @KINDS
+def test_decode_shows_what_is_not_a_number(dtype):
+    """A scale that is NaN, as a key or value that was not finite leaves it, and a query that is none: the heads that meet it are NaN,
+    wherever in the context it lies; others are as without it."""
+    from art_b200.ops import kv_q8
+
+    Hq, Hkv, hd, bs, lens = 6, 2, 64, 16, [3000, 40, 9]
+    g = torch.Generator(device=DEV).manual_seed(14)
+    bt, nb = pages(lens, bs)
+    cache = filled(nb, Hkv, bs, hd, dtype, g)
+    q = torch.randn(3, Hq * hd, generator=g, device=DEV).bfloat16()
+    table, ctx = bt.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ws = kv_q8.decode_q8_workspace(3, Hq, Hkv, hd, DEV)
+    good = kv_q8.paged_decode_q8(q, *cache, table, ctx, Hq, Hkv, hd, torch.empty_like(q), ws).clone()
+    cache[2][bt[0, 100], 1] = float("nan")         # a key scale amid the first context, kv head 1
+    cache[3][bt[1, 2], 0] = float("nan")           # a value scale at the end of the second, kv head 0
+    q[2, 5 * hd + 7] = float("nan")                # the last query head of the third
+    out = kv_q8.paged_decode_q8(q, *cache, table, ctx, Hq, Hkv, hd, torch.empty_like(q), ws)
+    bad = torch.zeros(3, Hq, dtype=torch.bool, device=DEV)
+    bad[0, 3:] = bad[1, :3] = bad[2, 5] = True
+    out, good = out.view(3, Hq, hd), good.view(3, Hq, hd)
+    assert out[bad].isnan().all() and torch.equal(out[~bad], good[~bad])
+
+
+@KINDS
 def test_a_sequence_from_prompt_to_decoding(dtype):
     """The calls in the order of a rollout: a prompt in two portions, the first read back for the second, then tokens one by one."""
     from art_b200.ops import kv_q8
