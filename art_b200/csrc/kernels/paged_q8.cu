@@ -26,14 +26,13 @@ constexpr int PQ_MIN_TILES = 4;   // tiles of a CTA at least: one per warp
 constexpr int PQ_ENTRIES = 1024;         // of a CTA's list of where sequences begin
 constexpr int PQ_ROUND = 16;             // tiles that a warp looks up at a time
 constexpr int PQ_NOTES = 2 * PQ_ROUND;   // and keeps noted: those in use and the next
-constexpr int PQ_BATCH = 4;              // parts of a sequence that are added up at a time
 constexpr float PQ_SLACK = 8.f;          // how far (in powers of two) a score may pass the reference before that moves
 
 __host__ __device__ constexpr int pq_heads(int G) { return G > 8 ? 16 : 8; }
 // tiles of a warp in shared memory
 __host__ __device__ constexpr int pq_stages(int hd, int heads) { return hd == 128 ? 2 : hd == 64 ? (heads == 8 ? 3 : 2) : 4; }
 __host__ __device__ constexpr int pq_ctas_per_sm(int hd) { return hd == 128 ? 2 : 3; }  // by shared memory
-__host__ __device__ constexpr int pq_piece_floats(int heads, int hd) { return heads * hd + ((2 * heads + 3) & ~3); }
+__host__ __device__ constexpr int pq_piece_floats(int heads, int hd) { return heads * hd + 2 * heads; }
 
 template <int HD, int HEADS>
 struct PqSmem {
@@ -118,27 +117,6 @@ __device__ __forceinline__ void pq_put(__nv_bfloat16* dst, const uint32_t* r) {
   }
 }
 
-// A weighted sum of pieces: eight values of a head, and the sum of its weights.
-struct PqSum {
-  float4 a, b;
-  float l;
-  __device__ __forceinline__ void add(const float4& x, const float4& y, float sum, float f) {
-    a = make_float4(fmaf(x.x, f, a.x), fmaf(x.y, f, a.y), fmaf(x.z, f, a.z), fmaf(x.w, f, a.w));
-    b = make_float4(fmaf(y.x, f, b.x), fmaf(y.y, f, b.y), fmaf(y.z, f, b.z), fmaf(y.w, f, b.w));
-    l = fmaf(sum, f, l);
-  }
-  __device__ __forceinline__ void scale(float f) {
-    a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
-    b = make_float4(b.x * f, b.y * f, b.z * f, b.w * f);
-    l *= f;
-  }
-  __device__ __forceinline__ void store(__nv_bfloat16* dst) const {
-    const float inv = l == 0.f ? 0.f : rcp_approx(l);
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv),
-                                                pack_bf16x2(b.x * inv, b.y * inv), pack_bf16x2(b.z * inv, b.w * inv));
-  }
-};
-
 // A tile: which of its sequence's it is; keys of each stretch (16, fewer at a context's end, 0 where its block is none), their rows
 // in the codes and their scales.
 struct __align__(16) PqNote {
@@ -152,13 +130,121 @@ struct PqPiece {
   int seq, len, first, lo, hi;
 };
 
+// not at all; to its end, and then others'; to its end, which is the warp's; beyond the warp's end
+enum PqGoesOn : int { PQ_NOT = 0, PQ_THEN_OTHERS = 1, PQ_TO_ITS_END = 2, PQ_BEYOND = 3 };
+
+// A piece as a warp's registers hold it, of the sums of some keys: heads n * 8 + 2t + x, values g * hd / 8 + 2j (acc[][][x]) and + 1
+// (acc[][][2 + x]), references and sums of weights.  In memory: a float4 per lane, lanes side by side, then references and sums by
+// head.
+template <int NT, int JT>
+struct PqSums {
+  float m[NT][2], l[NT][2], acc[NT][JT][4];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[n][x] = -INFINITY;
+        l[n][x] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[n][j][x] = 0.f;
+    }
+  }
+
+  template <bool GLOBAL>
+  __device__ __forceinline__ void put(float* dst, int lane, int G) const {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (GLOBAL && n * 8 + 2 * t >= G) continue;              // no such heads
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        float4* to = reinterpret_cast<float4*>(dst) + (n * JT + j) * 32 + lane;
+        const float4 v = make_float4(acc[n][j][0], acc[n][j][1], acc[n][j][2], acc[n][j][3]);
+        if (GLOBAL) __stcg(to, v);
+        else *to = v;
+      }
+      if (g == 0) {
+        float* tail = dst + NT * JT * 128 + n * 8 + 2 * t;
+        *reinterpret_cast<float2*>(tail) = make_float2(m[n][0], m[n][1]);
+        *reinterpret_cast<float2*>(tail + NT * 8) = make_float2(l[n][0], l[n][1]);
+      }
+    }
+  }
+
+  template <bool GLOBAL>
+  __device__ __forceinline__ void get(const float* src, int lane, int G) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (GLOBAL && n * 8 + 2 * t >= G) continue;
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        const float4* from = reinterpret_cast<const float4*>(src) + (n * JT + j) * 32 + lane;
+        const float4 v = GLOBAL ? __ldcg(from) : *from;
+        acc[n][j][0] = v.x;
+        acc[n][j][1] = v.y;
+        acc[n][j][2] = v.z;
+        acc[n][j][3] = v.w;
+      }
+      const float2* tail = reinterpret_cast<const float2*>(src + NT * JT * 128 + n * 8 + 2 * t);
+      const float2 a = GLOBAL ? __ldcg(tail) : tail[0], b = GLOBAL ? __ldcg(tail + NT * 4) : tail[NT * 4];
+      m[n][0] = a.x;
+      m[n][1] = a.y;
+      l[n][0] = b.x;
+      l[n][1] = b.y;
+    }
+  }
+
+  // Both are taken to the larger reference; what has none counts nothing, and sums that are not numbers stay so.
+  __device__ __forceinline__ void add(const PqSums& o) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float top = fmaxf(m[n][x], o.m[n][x]), r = top == -INFINITY ? 0.f : top;
+        const float a = pq_exp2(m[n][x] - r), b = pq_exp2(o.m[n][x] - r);
+        m[n][x] = top;
+        l[n][x] = l[n][x] * a + o.l[n][x] * b;
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          acc[n][j][x] = acc[n][j][x] * a + o.acc[n][j][x] * b;
+          acc[n][j][2 + x] = acc[n][j][2 + x] * a + o.acc[n][j][2 + x] * b;
+        }
+      }
+  }
+
+  // The heads' result, `unit` times the sums over the sums of weights; `o`: the first head's row.
+  __device__ __forceinline__ void write(__nv_bfloat16* o, float unit, int lane, int G) const {
+    constexpr int HD = JT * 16;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int head = n * 8 + 2 * t + x;
+        if (head >= G) continue;
+        const float f = l[n][x] == 0.f ? 0.f : unit * rcp_approx(l[n][x]);
+        uint32_t r[JT];
+#pragma unroll
+        for (int j = 0; j < JT; ++j) r[j] = pack_bf16x2(acc[n][j][x] * f, acc[n][j][2 + x] * f);
+        pq_put<JT * 4>(o + head * HD + g * (HD / 8), r);
+      }
+  }
+};
+
 // The sequences are laid end to end, in tiles of PQ_KEYS keys, and cut into equal shares, wherever sequences begin and end in
 // them; a share belongs to Hkv neighbouring CTAs, one per kv head, and the shares together fill the chip once.  A CTA's share is
 // cut again into four, one per warp, which goes through its tiles without a stop at the ends of sequences: its lanes look up
 // sixteen tiles at a time (sequence, blocks, then scales) while those before are in use, and a tile's copies into shared memory
 // start as soon as the warp has taken the last bytes of the one whose place it gets.  A sequence that one warp reads whole is
-// written by it.  The pieces of others meet in shared memory, and what still is a part then goes to the workspace; the CTA that
-// finishes last adds the parts up in their order.
+// written by it.  Of one that several warps of the CTA read, the first adds the others' pieces to its own; what still is a part then
+// goes to the workspace, and the CTA that finishes last adds the parts up, each warp every fourth, in an order that is always the
+// same.
 template <int KIND, int HD, int HEADS>
 __global__ void __launch_bounds__(PQ_THREADS, pq_ctas_per_sm(HD))
 paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -173,8 +259,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   uint8_t* rings = pq_smem_raw + (1024 - (smem_u32(pq_smem_raw) & 1023));
   __shared__ int s_warp[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES];
   __shared__ volatile int s_abort;
-  __shared__ PqPiece s_piece[2 * PQ_WARPS];
-  __shared__ int4 s_part[2];                // sequences that the CTA leaves a part of: number, first share, parts, 1: it is the last
+  __shared__ int s_goes_on[PQ_WARPS];       // how a warp goes on with the sequence that the one before it ends in (PqGoesOn)
+  __shared__ int4 s_part[2];                // sequences that the CTA is the last to finish a part of: number, first share, parts, 1
   __shared__ PqNote s_note[PQ_WARPS][PQ_NOTES];
   __shared__ __align__(8) uint64_t s_full[PQ_WARPS][STAGES];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -182,10 +268,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     mbar_init(&s_full[0][0] + tid, 1);
     fence_mbar_init();
   }
-  if (tid < 2 * PQ_WARPS) {
-    s_piece[tid].seq = -1;
-    if (tid < 2) s_part[tid] = make_int4(0, 0, 0, 0);
-  }
+  if (tid < PQ_WARPS) s_goes_on[tid] = PQ_NOT;
+  if (tid < 2) s_part[tid] = make_int4(0, 0, 0, 0);
   if (tid == PQ_THREADS - 1) {
     s_abort = 0;
     tma_prefetch_desc(&k_map);
@@ -264,6 +348,18 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __syncthreads();
 
   const int lo = at + warp * per_warp, tiles = min(end, lo + per_warp) - lo;
+  constexpr int SLOT = pq_piece_floats(HEADS, HD);
+  // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
+  auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * SLOT; };
+  auto result = [&](int seq) { return out + static_cast<size_t>(seq) * ldo + kvh * G * HD; };
+  auto piece_at = [&](int w) { return reinterpret_cast<float*>(rings + PQ_WARPS * S::RING + w * S::PIECE); };
+  auto ring_at = [&](int w) { return reinterpret_cast<float*>(rings + w * S::RING); };
+  PqSums<NT, JT> sums;
+  auto& m = sums.m;
+  auto& l = sums.l;
+  auto& acc = sums.acc;
+  PqPiece last, owed;            // the piece that the warp ends with, and the part that warp 0 leaves before
+  bool open = false, owes = false;
   if (tiles > 0) {
     uint8_t* ring = rings + warp * S::RING;
     PqNote* notes = s_note[warp];
@@ -341,7 +437,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int v_at[2] = {pq_piece_at<HD>(2 * t, v_piece) + v_rest, pq_piece_at<HD>(2 * t + 1, v_piece) + v_rest};
 
     uint32_t q_raw[NT][JT * 2], qf[NT][JT][2];
-    float qs[NT][2], m[NT][2], l[NT][2], acc[NT][JT][4], unit, per_unit;
+    float qs[NT][2], unit, per_unit;
     auto request_q = [&](int seq) {         // heads g (and g + 8), hd / 4 values: those that the lane holds of a key, in the same order
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -388,16 +484,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           const float down = scale_log2 * q8_pow2(-e);
           qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);          // of heads 2t and 2t + 1: the columns this lane gets
           qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            m[n][x] = -INFINITY;
-            l[n][x] = 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < JT; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[n][j][x] = 0.f;
         }
+        sums.clear();
       }
       const int stage = i % STAGES;
       const uint8_t* codes = ring + stage * S::STAGE;
@@ -570,176 +658,113 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
 
       if (i + 1 == tiles || ends) {
-        const bool whole = piece_lo == 0 && ends;
-        // the last piece goes where the tiles were
-        float* piece = reinterpret_cast<float*>(i + 1 == tiles ? ring : rings + PQ_WARPS * S::RING + warp * S::PIECE);
-        __syncwarp();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float sum = l[n][x];
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const int head = n * 8 + 2 * t + x;
-            const float f = whole ? (sum == 0.f ? 0.f : unit * rcp_approx(sum)) : unit;
-            if (whole) {
-              if (head < G) {
-                __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + (kvh * G + head) * HD + g * (HD / 8);
-                uint32_t o[JT];
+            for (int o = 4; o < 32; o <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], o);
+        if (piece_lo == 0 && ends) {
+          sums.write(result(seq), unit, lane, G);
+        } else {
 #pragma unroll
-                for (int j = 0; j < JT; ++j) o[j] = pack_bf16x2(acc[n][j][x] * f, acc[n][j][2 + x] * f);
-                pq_put<JT * 4>(o_row, o);
-              }
-            } else {
-              float* dst = piece + head * HD + g * (HD / 8);
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < JT; j += 2)
-                *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(acc[n][j][x] * f, acc[n][j][2 + x] * f, acc[n][j + 1][x] * f, acc[n][j + 1][2 + x] * f);
-              if (g == 0) {
-                piece[HEADS * HD + head] = m[n][x];
-                piece[HEADS * HD + HEADS + head] = sum;
-              }
-            }
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) acc[n][j][x] *= unit;
+          const PqPiece piece{seq, len, lo + i - tile, piece_lo, tile + 1};
+          if (i + 1 == tiles) {               // stays in registers
+            open = true;
+            last = piece;
+          } else if (warp == 0) {             // the end of a sequence that an earlier CTA begins
+            sums.template put<true>(slot(share, false), lane, G);
+            owes = true;
+            owed = piece;
+          } else {                            // the end of one that an earlier warp begins
+            sums.template put<false>(piece_at(warp), lane, G);
+            if (lane == 0) s_goes_on[warp] = PQ_THEN_OTHERS;
           }
-        if (!whole && lane == 0) s_piece[warp * 2 + (i + 1 == tiles)] = PqPiece{seq, len, lo + i - tile, piece_lo, tile + 1};
+        }
         piece_lo = 0;                         // the next sequence begins with the next tile
         fresh = true;
       }
     }
   }
   pdl_launch_dependents();
+  const bool follows = open && warp > 0 && last.lo > 0;        // a warp before this one begins it
+  if (follows) {
+    __syncwarp();
+    sums.template put<false>(ring_at(warp), lane, G);          // where its tiles were
+    if (lane == 0) s_goes_on[warp] = last.hi == tiles_in(last.len) ? PQ_TO_ITS_END : PQ_BEYOND;
+  }
   __syncthreads();
   if (s_abort) {                              // no copy may outlive the CTA
     if (lane < STAGES) mbar_wait_timed(&s_full[warp][lane], 0, 100), mbar_wait_timed(&s_full[warp][lane], 1, 100);
     return;
   }
-
-  // The pieces in their order: neighbours of one sequence, at most one per warp, are added up.
-  auto piece_of = [&](int p) {
-    return reinterpret_cast<const float*>(p & 1 ? rings + (p >> 1) * S::RING : rings + PQ_WARPS * S::RING + (p >> 1) * S::PIECE);
-  };
-  const int slot_floats = pq_piece_floats(G, HD), items = G * (HD / 8);           // a thread adds up 8 values of a head
-  // a CTA leaves at most two parts: of the sequence that it begins in the middle of, and of the one it ends in
-  auto slot = [&](int sh, bool starts) { return part + static_cast<size_t>((sh * Hkv + kvh) * 2 + starts) * slot_floats; };
-  // of a piece with reference m beside the largest of them, which is -inf where none has one; sums that are not numbers stay so
-  auto weight = [](float m, float top) { return pq_exp2(m - (top == -INFINITY ? 0.f : top)); };
-  const int my_seq = lane < 2 * PQ_WARPS ? s_piece[lane].seq : -1;
-  uint32_t todo = __ballot_sync(0xffffffffu, my_seq >= 0);
-  bool all_warps = false;                      // one sequence: all warps share its values; several: a warp for each
+  bool gives = false;
+  if (open && !follows) {
+    bool ended = last.hi == tiles_in(last.len);
 #pragma unroll 1
-  for (int k = 0; todo; ++k) {
-    const int p0 = __ffs(todo) - 1, seq = __shfl_sync(0xffffffffu, my_seq, p0);
-    const uint32_t mine = __ballot_sync(0xffffffffu, my_seq == seq);
-    todo &= ~mine;
-    if (k == 0) all_warps = todo == 0;
-    if (!all_warps && k % PQ_WARPS != warp) continue;
-    const PqPiece front = s_piece[p0];
-    const int hi = s_piece[31 - __clz(mine)].hi, tiles = tiles_in(front.len);
-    const bool whole = front.lo == 0 && hi == tiles;
-    const float* from[PQ_WARPS];
-    uint32_t rest = mine;
-#pragma unroll
-    for (int w = 0; w < PQ_WARPS; ++w) {
-      from[w] = rest ? piece_of(__ffs(rest) - 1) : nullptr;
-      rest &= rest - 1;
+    for (int w = warp + 1; w < PQ_WARPS && !ended; ++w) {
+      const int how = s_goes_on[w];
+      if (how == PQ_NOT) break;               // the CTA ends in it
+      PqSums<NT, JT> o;
+      o.template get<false>(how == PQ_THEN_OTHERS ? piece_at(w) : ring_at(w), lane, G);
+      sums.add(o);
+      ended = how != PQ_BEYOND;
     }
-    __nv_bfloat16* o_row = out + static_cast<size_t>(seq) * ldo + kvh * G * HD;
-    float* to = slot(share, front.lo == 0);
-#pragma unroll 1
-    for (int idx = all_warps ? tid : lane; idx < items; idx += all_warps ? PQ_THREADS : 32) {
-      const int r = idx / (HD / 8);
-      float m[PQ_WARPS], l[PQ_WARPS], top = -INFINITY;
-      PqSum sum{};
-#pragma unroll
-      for (int w = 0; w < PQ_WARPS; ++w) {
-        m[w] = from[w] ? from[w][HEADS * HD + r] : -INFINITY;
-        l[w] = from[w] ? from[w][HEADS * HD + HEADS + r] : 0.f;
-        top = fmaxf(top, m[w]);
-      }
-#pragma unroll
-      for (int w = 0; w < PQ_WARPS; ++w)
-        if (from[w]) {
-          const float4* v = reinterpret_cast<const float4*>(from[w]) + idx * 2;
-          sum.add(v[0], v[1], l[w], weight(m[w], top));
-        }
-      if (whole) {
-        sum.store(o_row + idx * 8);
-      } else {
-        __stcg(reinterpret_cast<float4*>(to) + idx * 2, sum.a);
-        __stcg(reinterpret_cast<float4*>(to) + idx * 2 + 1, sum.b);
-        if (idx * 8 == r * HD) {
-          __stcg(to + G * HD + r, top);
-          __stcg(to + G * HD + G + r, sum.l);
-        }
-      }
-    }
-    if (!whole && lane == 0 && (!all_warps || warp == 0)) {
-      const int sh0 = front.first / per;
-      s_part[front.lo == 0] = make_int4(seq, sh0, (front.first + tiles - 1) / per - sh0 + 1, 0);
+    if (ended && last.lo == 0) {
+      sums.write(result(last.seq), 1.f, lane, G);
+    } else {
+      sums.template put<true>(slot(share, last.lo == 0), lane, G);
+      gives = true;
     }
   }
-  __syncthreads();
-  if (warp < 2 && lane == 0 && s_part[warp].z > 0) {
-    int seen;                                                // releases what the CTA wrote before the barrier
-    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(&count[s_part[warp].x * Hkv + kvh]) : "memory");
-    s_part[warp].w = seen == s_part[warp].z - 1;
+  // lane 0: the part of a sequence that the CTA begins in the middle of, lane 1: of the one it ends in
+  const bool middle = owes || (gives && last.lo > 0);
+  __syncwarp();
+  if (lane == 0 ? middle : lane == 1 && gives && last.lo == 0) {
+    const PqPiece piece = lane == 0 && owes ? owed : last;
+    const int sh0 = piece.first / per, parts = (piece.first + tiles_in(piece.len) - 1) / per - sh0 + 1;
+    int seen;                                                  // releases what the warp wrote
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(&count[piece.seq * Hkv + kvh]) : "memory");
+    if (seen == parts - 1) s_part[lane] = make_int4(piece.seq, sh0, parts, 1);
   }
   __syncthreads();
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     if (!s_part[k].w) continue;
-    const int seq = s_part[k].x, parts = s_part[k].z;
-    const size_t stride = static_cast<size_t>(Hkv) * 2 * slot_floats;
-    const float* part0 = slot(s_part[k].y, false);           // the first part lies behind it, the others there
-    constexpr int N = PQ_BATCH;
-    struct Batch {
-      float m[N], l[N];
-      float4 a[N], b[N];
-    };
-    // the loads of parts q0, q0 + 1, ... for eight values of head r
-    auto request = [&](Batch& x, int q0, int r, int idx) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x.m[j] = -INFINITY;
-        x.l[j] = 0.f;
-        x.a[j] = x.b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (q0 + j < parts) {
-          const float* sl = part0 + (q0 + j) * stride + (q0 + j == 0 ? slot_floats : 0);
-          x.m[j] = __ldcg(sl + G * HD + r);
-          x.l[j] = __ldcg(sl + G * HD + G + r);
-          x.a[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2);
-          x.b[j] = __ldcg(reinterpret_cast<const float4*>(sl) + idx * 2 + 1);
-        }
-      }
-    };
-    auto add = [&](const Batch& x, PqSum& sum, float& top) {
-      float now = top;
-#pragma unroll
-      for (int j = 0; j < N; ++j) now = fmaxf(now, x.m[j]);
-      sum.scale(weight(top, now));
-      top = now;
-#pragma unroll
-      for (int j = 0; j < N; ++j) sum.add(x.a[j], x.b[j], x.l[j], weight(x.m[j], now));
-    };
+    const int seq = s_part[k].x, parts = s_part[k].z, stride = Hkv * 2 * SLOT;
+    const float* part0 = slot(s_part[k].y, false);             // the first part lies behind it, the others there
+    constexpr int BATCH = NT == 2 && HD > 32 ? 2 : NT * JT > 4 ? 3 : 4;      // parts whose loads are in flight, by registers
+    sums.clear();
 #pragma unroll 1
-    for (int idx = tid; idx < items; idx += PQ_THREADS) {
-      const int r = idx / (HD / 8);
-      float top = -INFINITY;
-      PqSum sum{};
-      Batch x, y;
-      request(x, 0, r, idx);
-#pragma unroll 1
-      for (int q0 = 0; q0 < parts; q0 += 2 * N) {          // the next batch is on its way while one is added up
-        if (q0 + N < parts) request(y, q0 + N, r, idx);
-        add(x, sum, top);
-        if (q0 + N >= parts) break;
-        if (q0 + 2 * N < parts) request(x, q0 + 2 * N, r, idx);
-        add(y, sum, top);
+    for (int p = warp; p < parts; p += PQ_WARPS * BATCH) {
+      PqSums<NT, JT> o[BATCH];
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int which = p + b * PQ_WARPS;
+        o[b].clear();
+        if (which < parts) o[b].template get<true>(part0 + static_cast<size_t>(which) * stride + (which == 0 ? SLOT : 0), lane, G);
       }
-      sum.store(out + static_cast<size_t>(seq) * ldo + kvh * G * HD + idx * 8);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) sums.add(o[b]);
     }
-    if (tid == 0) count[seq * Hkv + kvh] = 0;                // as the next launch expects it
+    if (warp > 0 && warp < parts) sums.template put<false>(piece_at(warp), lane, G);
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll 1
+      for (int w = 1; w < min(PQ_WARPS, parts); ++w) {
+        PqSums<NT, JT> o;
+        o.template get<false>(piece_at(w), lane, G);
+        sums.add(o);
+      }
+      sums.write(result(seq), 1.f, lane, G);
+      if (lane == 0) count[seq * Hkv + kvh] = 0;               // as the next launch expects it
+    }
+    __syncthreads();
   }
 }
 
@@ -750,7 +775,7 @@ static int pq_shares(int hd, int Hkv) {
 }
 
 static long pq_part_bytes(int Hq, int Hkv, int hd) {
-  return (static_cast<long>(pq_shares(hd, Hkv)) * Hkv * 2 * pq_piece_floats(Hq / Hkv, hd) * 4 + 15) / 16 * 16;
+  return static_cast<long>(pq_shares(hd, Hkv)) * Hkv * 2 * pq_piece_floats(pq_heads(Hq / Hkv), hd) * 4;
 }
 
 // The codes as rows of hd bytes, brought 16 at a time.
