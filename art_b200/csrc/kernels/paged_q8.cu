@@ -9,6 +9,16 @@
 // after a power of two per head that brings their largest to 2^14 (exact but for what is 2^-38 of it); weights are rounded to
 // fp16.  The order in which a product sums is free, so a lane's fragments are neighbouring bytes: hd / 4 values of a key, and
 // hd / 8 values of four keys, whose bytes are paired up in registers while they are widened.
+//
+// Bound by the cache's bytes, and beside them by what a launch begins and ends with.  256 contexts of 512 to 2032 keys, 28 / 4 heads
+// of 128, e4m3 (338 MB, 52 us at the copy rate): 61 us, of which 3 pass before the first keys are asked for and 6 between the ends of
+// the first and of the last warp's tiles; with the products left out 61 as well.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395
+// MB, 60 us): 70 us in bursts, 78 when the power cap has taken the clock to 1.77 GHz.  What else was tried on these two:
+//   80, 90   each lane loads its fragments from global memory into registers, three CTAs of four warps per SM
+//   72, 77   a fifth warp brings the tiles of the four, sixteen copies a turn from four lanes
+//   65, 75   one CTA of eight warps per SM
+//   71, 79   twice as many shares as fit the chip at a time
+//   137, 154 four CTAs per SM with 128 registers a thread
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
