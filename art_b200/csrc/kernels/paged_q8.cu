@@ -390,7 +390,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       next.seq = a * run;
       next.len = run == 1 ? s_len[a] : checked(ctx_len[next.seq]);
 #pragma unroll 1
-      while (x >= first + tiles_in(next.len)) {
+      while (x >= first + tiles_in(next.len) && next.seq + 1 < nseq) {
         first += tiles_in(next.len);
         next.len = checked(ctx_len[++next.seq]);
       }

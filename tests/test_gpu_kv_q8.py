@@ -442,6 +442,98 @@ def test_finish_kernel(dtype, M, Hq, Hkv, hd, bs, lora, norm, bias):
         assert torch.equal(a.float(), b.float())
 
 
+def order_case(g):
+    """Calls whose inputs another launch, copy or stream writes just before: ``(fill, calls, want)``."""
+    from art_b200.ops import kv_q8
+
+    Hq, Hkv, hd, bs, lens = 8, 2, 64, 16, [600, 33, 90, 1]
+    bt, nb = pages(lens, bs)
+    table = bt.to(DEV)
+    cache = filled(nb, Hkv, bs, hd, E4, g)
+    spare = [t.clone() for t in cache]
+    w, q0 = Hkv * hd, Hq * hd
+    slots = [int(bt[i, (n - 1) // bs]) * bs + (n - 1) % bs for i, n in enumerate(lens)]
+    src = (keys(4, Hkv, hd, g, spread=0.3, extra=q0), torch.tensor(slots, dtype=torch.int32, device=DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    x, slot, ctx = (torch.zeros_like(t) for t in src)
+    out, back = torch.zeros(4, q0, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 2 * w, dtype=torch.bfloat16, device=DEV)
+    ws = kv_q8.decode_q8_workspace(4, Hq, Hkv, hd, DEV)
+
+    def reset():
+        for a, b in zip(cache, spare):
+            a.copy_(b)
+        slot.fill_(-1)
+        for t in (x, ctx, out, back):
+            t.zero_()
+
+    def fill(copy=lambda a, b: a.copy_(b)):
+        for a, b in zip((x, slot, ctx), src):
+            copy(a, b)
+
+    def calls():
+        kv_q8.kv_write_q8(x, q0, q0 + w, slot, *cache)
+        kv_q8.paged_decode_q8(x, *cache, table, ctx, Hq, Hkv, hd, out, ws)
+        kv_q8.kv_rows_q8(*cache, slot, back, 0, w)
+
+    def got():
+        torch.cuda.synchronize()
+        return [t.clone() for t in (out, back, *(c.float() for c in cache))]
+
+    reset()
+    fill()
+    torch.cuda.synchronize()
+    calls()
+    return reset, fill, calls, got, got()
+
+
+@pytest.mark.parametrize("how", ["kernel", "copy", "stream", "graph", "forked graph"])
+def test_inputs_that_are_only_just_written(how):
+    """Launches start ahead of what comes before them; what they read is there all the same."""
+    g = torch.Generator(device=DEV).manual_seed(31)
+    reset, fill, calls, got, want = order_case(g)
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+
+    def same_as_wanted():
+        for a, b in zip(got(), want):
+            assert torch.equal(a, b)
+
+    def forked():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000)
+            fill()
+        torch.cuda._sleep(1000)
+        torch.cuda.current_stream().wait_stream(side)
+        calls()
+
+    for _ in range(3):
+        reset()
+        torch.cuda.synchronize()
+        if how == "kernel":
+            torch.cuda._sleep(200_000)
+            fill(lambda a, b: torch.add(b, 0, out=a))
+            calls()
+        elif how == "copy":
+            host = {}
+            fill(lambda a, b: host.__setitem__(a.data_ptr(), b.cpu().pin_memory()))
+            torch.cuda._sleep(200_000)
+            fill(lambda a, b: a.copy_(host[a.data_ptr()], non_blocking=True))
+            calls()
+        elif how == "stream":
+            forked()
+        else:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                if how == "graph":
+                    torch.cuda._sleep(200_000)
+                    fill()
+                    calls()
+                else:
+                    forked()
+            reset()
+            graph.replay()
+        same_as_wanted()
+
+
 def test_places_outside_the_cache_are_reported():
     """Slots, table entries and lengths that name no place are skipped or cut off, and the status word says so."""
     from art_b200.ops import _lib, kv_q8
