@@ -253,8 +253,7 @@ struct PqSums {
 // sixteen tiles at a time (sequence, blocks, then scales) while those before are in use, and a tile's copies into shared memory
 // start as soon as the warp has taken the last bytes of the one whose place it gets.  A sequence that one warp reads whole is
 // written by it.  Of one that several warps of the CTA read, the first adds the others' pieces to its own; what still is a part then
-// goes to the workspace, and the CTA that finishes last adds the parts up, each warp every fourth, in an order that is always the
-// same.
+// goes to the workspace, and the CTA that finishes last adds the parts up, in an order that is always the same.
 template <int KIND, int HD, int HEADS>
 __global__ void __launch_bounds__(PQ_THREADS, pq_ctas_per_sm(HD))
 paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -749,32 +748,40 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int seq = s_part[k].x, parts = s_part[k].z, stride = Hkv * 2 * SLOT;
     const float* part0 = slot(s_part[k].y, false);             // the first part lies behind it, the others there
     constexpr int BATCH = NT == 2 && HD > 32 ? 2 : NT * JT > 4 ? 3 : 4;      // parts whose loads are in flight, by registers
+    // few parts are one warp's, the two sequences' then two warps'
+    const int team = min(PQ_WARPS, (parts + BATCH - 1) / BATCH), me = (warp + PQ_WARPS - k) % PQ_WARPS;
     sums.clear();
+    if (me < team) {
 #pragma unroll 1
-    for (int p = warp; p < parts; p += PQ_WARPS * BATCH) {
-      PqSums<NT, JT> o[BATCH];
+      for (int p = me; p < parts; p += team * BATCH) {
+        PqSums<NT, JT> o[BATCH];
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int which = p + b * PQ_WARPS;
-        o[b].clear();
-        if (which < parts) o[b].template get<true>(part0 + static_cast<size_t>(which) * stride + (which == 0 ? SLOT : 0), lane, G);
+        for (int b = 0; b < BATCH; ++b) {
+          const int which = p + b * team;
+          o[b].clear();
+          if (which < parts) o[b].template get<true>(part0 + static_cast<size_t>(which) * stride + (which == 0 ? SLOT : 0), lane, G);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) sums.add(o[b]);
       }
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) sums.add(o[b]);
     }
-    if (warp > 0 && warp < parts) sums.template put<false>(piece_at(warp), lane, G);
-    __syncthreads();
-    if (warp == 0) {
+    if (team > 1) {
+      if (me > 0 && me < team) sums.template put<false>(piece_at(me), lane, G);
+      __syncthreads();
+      if (me == 0) {
 #pragma unroll 1
-      for (int w = 1; w < min(PQ_WARPS, parts); ++w) {
-        PqSums<NT, JT> o;
-        o.template get<false>(piece_at(w), lane, G);
-        sums.add(o);
+        for (int w = 1; w < team; ++w) {
+          PqSums<NT, JT> o;
+          o.template get<false>(piece_at(w), lane, G);
+          sums.add(o);
+        }
       }
+    }
+    if (me == 0) {
       sums.write(result(seq), 1.f, lane, G);
       if (lane == 0) count[seq * Hkv + kvh] = 0;               // as the next launch expects it
     }
-    __syncthreads();
+    if (team > 1) __syncthreads();
   }
 }
 
