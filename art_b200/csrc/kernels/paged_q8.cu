@@ -5,15 +5,20 @@
 // read once for all of them.  Both products have the cache's side as their rows,
 //     S^T [16 keys x heads] = K Q^T,     O^T [hd x heads] = V^T P^T,
 // and 16 keys are always of one block: a key scale is one factor of a tile of scores, a value scale one of a tile of weights, and
-// no code is ever multiplied by either.  Codes become fp16 (exact: e4m3 and int8 have at most 8 significant bits), queries too,
-// after a power of two per head that brings their largest to 2^14 (exact but for what is 2^-38 of it); weights are rounded to
-// fp16.  The order in which a product sums is free, so a lane's fragments are neighbouring bytes: hd / 4 values of a key, and
-// hd / 8 values of four keys, whose bytes are paired up in registers while they are widened.
+// no code is ever multiplied by either.  Codes become fp16 (exact: e4m3 and int8 have at most 8 significant bits) but for keys in
+// int8, which are multiplied as they are.  A power of two per head brings the largest of its query to [2^14, 2^15); beside e4m3 keys
+// queries are fp16 then (exact but for what is 2^-38 of the largest), beside int8 keys whole numbers of 16 bits (off by 1/2 at most:
+// 2^-15 of the largest, where a key's code is off by 2^-8 of its block's largest), whose high and low bytes have a product each, in
+// exact sums.  Widening int8 keys instead took 70.5 us where this takes 66 (the 48 contexts below); four e4m3 codes are widened by
+// two instructions where int8 takes five.  Weights are rounded to fp16.  The order in which a product sums is free, so a lane's
+// fragments are neighbouring bytes: hd / 4 values of a key, and hd / 8 values of four keys, whose bytes are paired up in registers
+// while they are widened.
 //
 // Bound by the cache's bytes, and beside them by what a launch begins and ends with.  256 contexts of 512 to 2032 keys, 28 / 4 heads
-// of 128, e4m3 (338 MB, 52 us at the copy rate): 61 us, of which 3 pass before the first keys are asked for and 6 between the ends of
-// the first and of the last warp's tiles; with the products left out 61 as well.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395
-// MB, 60 us): 70 us in bursts, 78 when the power cap has taken the clock to 1.77 GHz.  What else was tried on these two:
+// of 128, e4m3 (338 MB, 52 us at the copy rate): 60 us, of which 3 pass before the first keys are asked for and 6 between the ends of
+// the first and of the last warp's tiles.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395 MB, 60 us): 66 us in bursts, 69 when
+// the power cap has taken the clock to 1.85 GHz.  What else was tried on these two,
+// when they took 61 and 70:
 //   80, 90   each lane loads its fragments from global memory into registers, three CTAs of four warps per SM
 //   72, 77   a fifth warp brings the tiles of the four, sixteen copies a turn from four lanes
 //   65, 75   one CTA of eight warps per SM
@@ -98,6 +103,20 @@ __device__ __forceinline__ void pq_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 32 int8 codes of 16 keys, as they lie in the cache, with the high bytes of the queries or, UNSIGNED, the low ones.  Each sum is
+// below 128 * 255 * 128 and the two together below 2^30.
+template <bool UNSIGNED>
+__device__ __forceinline__ void pq_mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (UNSIGNED)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t pq_transpose(uint32_t x) {       // an 8 x 8 tile of 16-bit numbers over the warp
@@ -486,11 +505,26 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           const int e = top >= 0x7f80u || top == 0 ? 0 : min(100, 14 + 127 - static_cast<int>(top >> 7));
           const float up = q8_pow2(e);
 #pragma unroll
-          for (int j = 0; j < JT; ++j)
+          for (int j = 0; j < JT; ++j) {
+            float v[4];
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              qf[n][j][x] = pq_half2(__uint_as_float(raw[2 * j + x] << 16) * up, __uint_as_float(raw[2 * j + x] & 0xffff0000u) * up);
-          const float down = scale_log2 * q8_pow2(-e);
+            for (int x = 0; x < 2; ++x) {
+              v[2 * x] = __uint_as_float(raw[2 * j + x] << 16) * up;
+              v[2 * x + 1] = __uint_as_float(raw[2 * j + x] & 0xffff0000u) * up;
+            }
+            if constexpr (KIND == Q8_INT8) {         // whole numbers of 16 bits, by bytes: high ones and low ones of four
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) w[x] = __float_as_uint(v[x] + 12582912.f);
+              const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+              qf[n][j][0] = __byte_perm(a, b, 0x7632);
+              qf[n][j][1] = __byte_perm(a, b, 0x5410);
+            } else {
+              qf[n][j][0] = pq_half2(v[0], v[1]);
+              qf[n][j][1] = pq_half2(v[2], v[3]);
+            }
+          }
+          const float down = top >= 0x7f80u ? NAN : scale_log2 * q8_pow2(-e);       // whole numbers keep no NaN, nor an infinity
           qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);          // of heads 2t and 2t + 1: the columns this lane gets
           qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
         }
@@ -527,17 +561,31 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             if (HD == 128) pq_take<16>(kr[r] + KW / 2, p + k_at[1]);
           }
         }
+        if constexpr (KIND == Q8_INT8) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[u][n][x] = 0.f;
+            for (int j = 0; j < JT; j += 2) {
+              pq_mma_s8<false>(hi, kr[0][j], kr[1][j], kr[0][j + 1], kr[1][j + 1], qf[n][j][0], qf[n][j + 1][0]);
+              pq_mma_s8<true>(lo, kr[0][j], kr[1][j], kr[0][j + 1], kr[1][j + 1], qf[n][j][1], qf[n][j + 1][1]);
+            }
 #pragma unroll
-        for (int j = 0; j < JT; ++j) {
-          uint32_t a0, a1, a2, a3;
-          pq_widen<KIND>(kr[0][j], a0, a2);
-          pq_widen<KIND>(kr[1][j], a1, a3);
+            for (int x = 0; x < 4; ++x) s[u][n][x] = static_cast<float>(hi[x] * 256 + lo[x]);
+          }
+        } else {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) pq_mma(s[u][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[u][n][x] = 0.f;
+#pragma unroll
+          for (int j = 0; j < JT; ++j) {
+            uint32_t a0, a1, a2, a3;
+            pq_widen<KIND>(kr[0][j], a0, a2);
+            pq_widen<KIND>(kr[1][j], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) pq_mma(s[u][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
+          }
         }
       }
       uint32_t vr[2][4][VW];

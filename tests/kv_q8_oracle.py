@@ -56,9 +56,10 @@ class Cache:
         return torch.where((s >= 0)[:, None, None], v, torch.zeros_like(v))
 
 
-def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dtype=None):
     """``q`` [Hq, hd] over ``k``, ``v`` [n, Hkv, hd], all float64: the result [Hq, hd] and how far a kernel may be from it that
-    takes products of exact operands into fp32 sums, rounds each weight to fp16 and the result to bf16."""
+    takes products of exact operands into fp32 sums, rounds each weight to fp16 and the result to bf16; for codes of ``dtype`` int8
+    one that first rounds a head's query to 16-bit whole numbers, the largest of which is at least 2^14."""
     Hq, hd = q.shape
     G, n = Hq // k.shape[1], k.shape[0]
     if n == 0:
@@ -71,6 +72,10 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     # is good to 2^-21; numerator and denominator have both errors.  Sums over n keys: rounded n times in each of few orders, which
     # 2^-24 * n bounds.  A weight (at most 2^8 above the running reference, whose own is 1) below 2^-14 is rounded by 2^-25.
     score = (hd + 4) * 2.0 ** -24 * float((torch.einsum("hd,nhd->hn", q.abs(), k.abs()) / math.sqrt(hd)).max()) + 2.0 ** -21
+    if dtype == torch.int8:
+        # value i of a query is off by 1/2 where the largest is 2^14 or more, so by 2^-15 max|q|, and the score by the sum over i of
+        # that times |k_i|
+        score += 2.0 ** -15 * float((q.abs().amax(1)[:, None] * k.abs().sum(-1).T).max()) / math.sqrt(hd)
     weight = 2.0 ** -11 + 2 * score + 2 * n * 2.0 ** -24
     bound = 2.0 ** -8 * ref.abs() + 1.01 * weight * (size + ref.abs()) + 2.0 ** -25 * v.abs().sum(0)
     return ref, bound + 1e-30

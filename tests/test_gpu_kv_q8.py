@@ -193,7 +193,7 @@ def check_decode(out, q, cache, bt, lens, Hq, hd, some=16):
         n = lens[i]
         t = torch.arange(n)
         slots = bt[i].cpu().long()[t // bs] * bs + t % bs
-        ref, bound = attend(q[i, :Hq * hd].double().cpu().view(Hq, hd), k.tokens(slots), v.tokens(slots))
+        ref, bound = attend(q[i, :Hq * hd].double().cpu().view(Hq, hd), k.tokens(slots), v.tokens(slots), k.dtype)
         off = (out[i, :Hq * hd].double().cpu().view(Hq, hd) - ref).abs()
         assert (off <= bound).all(), (i, n, float((off - bound).max()))
 
@@ -260,6 +260,31 @@ def test_decode_sharp_and_large_scores(dtype):
         q[0, 5] *= 2.0 ** -20
         out = kv_q8.paged_decode_q8(q, *cache, bt, ctx, Hq, Hkv, hd, torch.empty_like(q), ws)
         check_decode(out, q, cache, bt, lens, Hq, hd)
+
+
+@KINDS
+@pytest.mark.parametrize("Hq,Hkv,hd", [(4, 2, 32), (6, 2, 64), (28, 4, 128), (16, 1, 128)])
+def test_decode_queries_of_uneven_size(dtype, Hq, Hkv, hd):
+    """Queries of one value among zeros, of values from the largest a head's scaling leaves to bits below its last, of all the same
+    largest magnitude, of bf16's smallest numbers, and of zeros: the rounding of a query is relative to its head."""
+    from art_b200.ops import kv_q8
+
+    bs, lens = 16, [700, 33, 64, 90, 500]
+    g = torch.Generator(device=DEV).manual_seed(21)
+    bt, nb = pages(lens, bs)
+    cache = filled(nb, Hkv, bs, hd, dtype, g)
+    q = torch.randn(len(lens), Hq, hd, generator=g, device=DEV)
+    q[0] = 0
+    q[0, :, 5] = torch.linspace(-3, 3, Hq, device=DEV)
+    q[1] *= torch.exp2(-(torch.arange(hd, device=DEV) % 24).float())
+    q[2] = q[2].sign() * 255 * 2.0 ** -10
+    q[3] *= 2.0 ** -130
+    q[4, ::2] = 0
+    q = q.bfloat16().view(len(lens), Hq * hd)
+    table, ctx = bt.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ws = kv_q8.decode_q8_workspace(len(lens), Hq, Hkv, hd, DEV)
+    out = kv_q8.paged_decode_q8(q, *cache, table, ctx, Hq, Hkv, hd, torch.empty_like(q), ws)
+    check_decode(out, q, cache, bt, lens, Hq, hd)
 
 
 def test_decode_keeps_what_is_masked_out():

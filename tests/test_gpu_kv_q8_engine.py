@@ -135,7 +135,7 @@ def test_decode_steps(kind, n, hd, qk_norm, finish, monkeypatch):
             caches.append(now)
         for i in range(0, n, max(1, n // 10)):
             at = slots_of(seqs[i], len(seqs[i].tokens))
-            ref, bound = attend(st["q"][i].double().cpu().view(cfg.num_heads, hd), caches[0].tokens(at), caches[1].tokens(at))
+            ref, bound = attend(st["q"][i].double().cpu().view(cfg.num_heads, hd), caches[0].tokens(at), caches[1].tokens(at), caches[0].dtype)
             assert ((st["attn_out"][i].double().cpu().view(cfg.num_heads, hd) - ref).abs() <= bound).all()
     a, b = q8.decode(seqs, 16)[0], bf.decode(seqs, 16)[0]
     assert a == b
