@@ -9,16 +9,16 @@
 // int8, which are multiplied as they are.  A power of two per head brings the largest of its query to [2^14, 2^15); beside e4m3 keys
 // queries are fp16 then (exact but for what is 2^-38 of the largest), beside int8 keys whole numbers of 16 bits (off by 1/2 at most:
 // 2^-15 of the largest, where a key's code is off by 2^-8 of its block's largest), whose high and low bytes have a product each, in
-// exact sums.  Widening int8 keys instead took 70.5 us where this takes 66 (the 48 contexts below); four e4m3 codes are widened by
-// two instructions where int8 takes five.  Weights are rounded to fp16.  The order in which a product sums is free, so a lane's
-// fragments are neighbouring bytes: hd / 4 values of a key, and hd / 8 values of four keys, whose bytes are paired up in registers
-// while they are widened.
+// exact sums.  Widening int8 keys instead takes 70.5 us where this takes 66.8 (the 48 contexts below), under the power cap 77 and 73;
+// four e4m3 codes are widened by two instructions where int8 takes five.  Weights are rounded to fp16.  The order in which a product
+// sums is free, so a lane's fragments are neighbouring bytes: hd / 4 values of a key, and hd / 8 values of four keys, whose bytes are
+// paired up in registers while they are widened.
 //
 // Bound by the cache's bytes, and beside them by what a launch begins and ends with.  256 contexts of 512 to 2032 keys, 28 / 4 heads
 // of 128, e4m3 (338 MB, 52 us at the copy rate): 60 us, of which 3 pass before the first keys are asked for and 6 between the ends of
-// the first and of the last warp's tiles.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395 MB, 60 us): 66 us in bursts, 69 when
-// the power cap has taken the clock to 1.85 GHz.  What else was tried on these two,
-// when they took 61 and 70:
+// the first and of the last warp's tiles.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395 MB, 60 us): 66 us in bursts, 69 to
+// 73, by the GPU, when the power cap has taken the clock to 1.85 or 1.75 GHz.  What else was tried on these two, when they took 61 and
+// 70:
 //   80, 90   each lane loads its fragments from global memory into registers, three CTAs of four warps per SM
 //   72, 77   a fifth warp brings the tiles of the four, sixteen copies a turn from four lanes
 //   65, 75   one CTA of eight warps per SM
