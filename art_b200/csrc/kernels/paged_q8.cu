@@ -701,14 +701,14 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (!(vs[u] >= 0.5f * unit && vs[u] <= 64.f * unit) && vs[u] != 0.f) {
-          const float f = fminf(unit * rcp_approx(vs[u]), 0x1p90f);        // beside sums that large a weight is nothing
+          const float f = fminf(unit * rcp_approx(vs[u]), 0x1p80f);        // beside sums that large a weight is nothing
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < JT; ++j)
 #pragma unroll
               for (int x = 0; x < 4; ++x) acc[n][j][x] *= f;
-          unit = f < 0x1p90f ? vs[u] : unit * 0x1p-90f;
+          unit = f < 0x1p80f ? vs[u] : unit * 0x1p-80f;
           per_unit = rcp_approx(unit);
         }
         add(u);
@@ -879,6 +879,8 @@ ARTB_EXPORT int artb_paged_decode_q8(const PagedDecodeArgs* args, cudaStream_t s
        reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
     return ERR_BAD_ALIGN;
   if (num_blocks * Hkv * block_size > 0x7fffffffL) return ERR_TOO_LARGE;        // rows are numbered with 31 bits
+  const long most = static_cast<long>(max_blocks) * block_size;                 // keys of a context, and so are all tiles
+  if ((((most < 0x7fffffffL ? most : 0x7fffffffL) + PQ_KEYS - 1) / PQ_KEYS) * num_seqs > 0x7f000000L) return ERR_TOO_LARGE;
   int dev_ = 0;
   if (cudaGetDevice(&dev_) != cudaSuccess || dev_ < 0 || dev_ >= 64) return ERR_BAD_SHAPE;
   const float scale_log2 = 1.4426950408889634f / sqrtf((float)hd);

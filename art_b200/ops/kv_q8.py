@@ -193,6 +193,14 @@ def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
             v_scale.data_ptr(), nb, n, ld, k_col, v_col, hkv, hd, bs, kind)
 
 
+def _meet(a: int, lda: int, b: int, ldb: int, n: int, width: int) -> bool:
+    """Whether ``n`` rows of ``width`` 16-bit numbers at address ``a`` and as many at ``b`` may share bytes; of rows of one stride
+    that lie among each other, whether they do."""
+    if b >= a + 2 * (lda * (n - 1) + width) or a >= b + 2 * (ldb * (n - 1) + width):
+        return False
+    return lda != ldb or not 2 * width <= (b - a) % (2 * ldb) <= 2 * (ldb - width)
+
+
 @functools.lru_cache(maxsize=1024)
 def _decode_bytes(n: int, Hq: int, Hkv: int, hd: int, device: int) -> int:
     with torch.cuda.device(device):
@@ -218,7 +226,8 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
     n, ldq = _rows("q", q, 0, 0, Hq * hd)
     m, ldo = _rows("out", out, 0, 0, Hq * hd)
-    if m != n or ldo < Hq * hd or (n and out.data_ptr() == q.data_ptr()):
+    at, to = q.data_ptr(), out.data_ptr()
+    if m != n or ldo < Hq * hd or (abs(to - at) < 2 * n * max(ldq, ldo) and _meet(at, ldq, to, ldo, n, Hq * hd)):
         raise ValueError(f"out must have {n} rows that do not overlap, nor lie where q does")
     _index("ctx_len", ctx_len, n)
     table = block_table.shape
@@ -227,6 +236,6 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     dev = _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
     if n and (ws.nbytes < _decode_bytes(n, Hq, Hkv, hd, dev) or not ws.is_contiguous()):
         raise ValueError(f"workspace of {ws.nbytes} bytes, {_decode_bytes(n, Hq, Hkv, hd, dev)} needed in a row")
-    _launch(dev, "artb_paged_decode_q8", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            block_table.data_ptr(), ctx_len.data_ptr(), out.data_ptr(), ws.data_ptr(), nb, n, ldq, ldo, Hq, Hkv, hd, bs, table[1], kind)
+    _launch(dev, "artb_paged_decode_q8", at, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), ctx_len.data_ptr(), to, ws.data_ptr(), nb, n, ldq, ldo, Hq, Hkv, hd, bs, table[1], kind)
     return out

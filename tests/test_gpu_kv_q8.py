@@ -263,6 +263,29 @@ def test_decode_sharp_and_large_scores(dtype):
 
 
 @KINDS
+@pytest.mark.parametrize("least,most", [(-110, 110), (-110, -90), (90, 110)])
+def test_decode_values_of_any_size(dtype, least, most):
+    """Blocks of values from bf16's smallest to its largest in one context, and blocks of zeros, whose scale is the least there is."""
+    from art_b200.ops import kv_q8
+
+    Hq, Hkv, hd, bs, lens = 8, 2, 64, 16, [3000, 37, 160]
+    g = torch.Generator(device=DEV).manual_seed(31)
+    bt, nb = pages(lens, bs)
+    bt = bt.to(DEV)
+    cache = empty(nb, Hkv, bs, hd, dtype)
+    x = torch.randn(nb * bs, 2 * Hkv * hd, generator=g, device=DEV)
+    size = torch.exp2(torch.randint(least, most + 1, (nb, 1), generator=g, device=DEV).float())
+    size[torch.rand(nb, generator=g, device=DEV) < 0.2] = 0
+    x[:, Hkv * hd:] *= size.repeat_interleave(bs, 0)
+    kv_q8.kv_write_q8(x.bfloat16(), 0, Hkv * hd, torch.arange(nb * bs, dtype=torch.int32, device=DEV), *cache)
+    ctx, ws = torch.tensor(lens, dtype=torch.int32, device=DEV), kv_q8.decode_q8_workspace(3, Hq, Hkv, hd, DEV)
+    for sharp in (1.0, 20.0):
+        q = (sharp * torch.randn(3, Hq * hd, generator=g, device=DEV)).bfloat16()
+        out = kv_q8.paged_decode_q8(q, *cache, bt, ctx, Hq, Hkv, hd, torch.empty_like(q), ws)
+        check_decode(out, q, cache, bt, lens, Hq, hd)
+
+
+@KINDS
 @pytest.mark.parametrize("Hq,Hkv,hd", [(4, 2, 32), (6, 2, 64), (28, 4, 128), (16, 1, 128)])
 def test_decode_queries_of_uneven_size(dtype, Hq, Hkv, hd):
     """Queries of one value among zeros, of values from the largest a head's scaling leaves to bits below its last, of all the same
@@ -656,3 +679,15 @@ def test_workspace_of_another_size_is_refused():
     bt, ctx = torch.zeros(300, 2, dtype=torch.int32, device=DEV), torch.zeros(300, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="needed"):
         kv_q8.paged_decode_q8(q, *cache, bt, ctx, 8, 2, 64, torch.empty_like(q), torch.zeros(8, dtype=torch.uint8, device=DEV))
+
+
+def test_more_tiles_than_can_be_numbered_are_refused():
+    from art_b200.ops import kv_q8
+
+    cache = empty(1, 1, 1 << 20, 32, E4)
+    q = torch.zeros(33, 32, dtype=torch.bfloat16, device=DEV)
+    bt, ctx = torch.zeros(33, 2048, dtype=torch.int32, device=DEV), torch.ones(33, dtype=torch.int32, device=DEV)
+    ws = kv_q8.decode_q8_workspace(33, 1, 1, 32, DEV)
+    with pytest.raises(ValueError, match="beyond the supported maximum"):
+        kv_q8.paged_decode_q8(q, *cache, bt, ctx, 1, 1, 32, torch.empty_like(q), ws)
+    kv_q8.paged_decode_q8(q, *cache, bt[:, :1024].contiguous(), ctx, 1, 1, 32, torch.empty_like(q), ws)

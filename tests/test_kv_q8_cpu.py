@@ -22,7 +22,7 @@ def rows(c, dst=None, slot=None, k_col=0, v_col=128):
     kv_q8.kv_rows_q8(*c, torch.zeros(3, dtype=torch.int32) if slot is None else slot, dst, k_col, v_col)
 
 
-SAME = torch.zeros(3, 256, dtype=BF)
+SAME, FUSED = torch.zeros(3, 256, dtype=BF), torch.zeros(4, 512, dtype=BF)
 
 
 def decode(c, q=None, table=None, ctx=None, heads=(4, 2, 64), out=None, ws=None):
@@ -87,6 +87,12 @@ def test_rows(kw, says):
     (dict(out=torch.zeros(2, 256, dtype=BF)), "out must have 3 rows"),
     (dict(out=torch.zeros(1, 256, dtype=BF).expand(3, 256)), "overlap"),
     (dict(q=SAME, out=SAME), "nor lie where q does"),
+    (dict(q=FUSED[:3, :256], out=FUSED[:3, 248:504]), "nor lie where q does"),
+    (dict(q=FUSED[:3, 256:], out=FUSED[:3, 8:264]), "nor lie where q does"),
+    (dict(q=FUSED[:3, :256], out=FUSED[1:, :256]), "nor lie where q does"),       # the next row's query
+    (dict(q=FUSED[:3, :256], out=FUSED.view(8, 256)[1:4]), "nor lie where q does"),
+    (dict(q=FUSED[:3, :256], out=FUSED[:3, 256:]), "one CUDA device"),            # beside it: in order
+    (dict(q=FUSED[:3, 256:], out=FUSED[1:, :256]), "one CUDA device"),
     (dict(table=torch.zeros(2, 2, dtype=torch.int32)), "block_table"),
     (dict(table=torch.zeros(3, 0, dtype=torch.int32)), "block_table"),
     (dict(table=torch.zeros(3, 2)), "block_table"),
