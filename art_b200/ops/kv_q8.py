@@ -35,6 +35,7 @@ _sigs = {
 }
 _bound: dict[str, object] = {}
 
+BF16, I32, F32 = torch.bfloat16, torch.int32, torch.float32
 KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 HEAD_DIMS = (32, 64, 128)
 
@@ -83,26 +84,32 @@ def _geometry(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int, i
         nb, hkv, bs, hd = shape
         scales = (nb, hkv)
         if (nb > 0 and hkv > 0 and bs > 0 and bs % 16 == 0 and hd in HEAD_DIMS and k_scale.shape == scales and v_scale.shape == scales
-                and k_scale.dtype is v_scale.dtype is torch.float32 and k_cache.is_contiguous() and v_cache.is_contiguous()
+                and k_scale.dtype is v_scale.dtype is F32 and k_cache.is_contiguous() and v_cache.is_contiguous()
                 and k_scale.is_contiguous() and v_scale.is_contiguous()):
             return nb, hkv, bs, hd, kind
     _check_cache(k_cache, v_cache, k_scale, v_scale)
 
 
-def _rows(name: str, x: torch.Tensor, lo: int, hi: int, width: int) -> tuple[int, int]:
-    """(rows, row stride) of ``x`` [rows, ld] bf16 that holds ``width`` columns from ``lo`` and from ``hi`` on, in pieces of 16 bytes."""
-    shape, stride = x.shape, x.stride()
-    if len(shape) != 2 or x.dtype is not torch.bfloat16 or (stride[1] != 1 and shape[1] > 1):
-        raise ValueError(f"{name} must be bf16 [rows, columns] with unit inner stride")
-    if lo < 0 or hi < 0 or lo % 8 or hi % 8 or max(lo, hi) + width > shape[1]:
-        raise ValueError(f"{name} [{shape[0]}, {shape[1]}] does not hold {width} columns at {lo} and {hi}, multiples of 8")
-    if (stride[0] % 8 and shape[0] > 1) or x.data_ptr() % 16:
-        raise ValueError(f"{name}: rows must begin on 16 bytes")
-    return shape[0], stride[0] if shape[0] > 1 else shape[1] + -shape[1] % 8
+def _rows(name: str, x: torch.Tensor, lo: int, hi: int, width: int) -> tuple[int, int, int]:
+    """(rows, row stride, address) of ``x`` [rows, ld] bf16 that holds ``width`` columns from ``lo`` and from ``hi`` on, in pieces of
+    16 bytes."""
+    shape, stride, at = x.shape, x.stride(), x.data_ptr()
+    if len(shape) == 2 and x.dtype is BF16:
+        n, cols = shape
+        ld, inner = stride
+        if n < 2:                              # a stride that leads nowhere
+            ld = cols + -cols % 8
+        if inner == 1 and not (lo | hi | ld) & 7 and not at & 15 and lo >= 0 and hi >= 0 and lo + width <= cols and hi + width <= cols:
+            return n, ld, at
+        if inner == 1:
+            if lo < 0 or hi < 0 or lo % 8 or hi % 8 or max(lo, hi) + width > cols:
+                raise ValueError(f"{name} [{n}, {cols}] does not hold {width} columns at {lo} and {hi}, multiples of 8")
+            raise ValueError(f"{name}: rows must begin on 16 bytes")
+    raise ValueError(f"{name} must be bf16 [rows, columns] with unit inner stride")
 
 
 def _index(name: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not I32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}]")
 
 
@@ -120,11 +127,8 @@ def _launch(dev: int, name: str, *args) -> None:
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _launch(dev, name, *args)
-    fn, block, word = _bound.get(name) or _f(name), _blocks.get(name), _lib.status_word(dev).data_ptr()
-    if block is not None:
-        rc = fn(block.pack(word, *args), _lib.raw_stream(dev))
-    else:
-        rc = fn(*args, word, _lib.raw_stream(dev))
+    fn, word, stream = _bound.get(name) or _f(name), _lib.status_word(dev).data_ptr(), _lib.raw_stream(dev)
+    rc = fn(_blocks[name].pack(word, *args), stream) if name in _blocks else fn(*args, word, stream)
     if rc:
         _lib.check_rc(rc, name.removeprefix("artb_"))
     _lib.LAUNCHES += 1
@@ -141,10 +145,12 @@ def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k
     codes.  A row at a block's first place starts the block anew.  Rows at later places can only raise the scale, and then what
     the block holds already is rounded once more.  A value that is not finite makes the scale NaN until the block starts anew."""
     nb, hkv, bs, hd, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
-    n, ld = _rows("qkv", qkv, k_col, v_col, hkv * hd)
+    n, ld, at = _rows("qkv", qkv, k_col, v_col, hkv * hd)
     _index("slot", slot, n)
-    dev = _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_write_q8", qkv.data_ptr(), slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+    dev = qkv.get_device()
+    if not (0 <= dev == slot.get_device() == k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device()):
+        _device(qkv, slot, k_cache, v_cache, k_scale, v_scale)
+    _launch(dev, "artb_kv_write_q8", at, slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), nb, n, ld, k_col, v_col, hkv, hd, bs, kind)
 
 
@@ -161,15 +167,15 @@ def decode_finalize_qkv_q8(ws: torch.Tensor, M: int, Hq: int, Hkv: int, hd: int,
         raise ValueError(f"{Hq} query heads and {Hkv} kv heads of {hd}: the cache has {hkv} of {d}, and the number of both must be even")
     _index("slot", slot, M)
     _index("pos", pos, M)
-    n, ldq = _rows("q_out", q_out, 0, 0, Hq * hd)
+    n, ldq, to = _rows("q_out", q_out, 0, 0, Hq * hd)
     N = (Hq + 2 * Hkv) * hd
-    if ws.dtype is not torch.float32 or ws.dim() != 2 or ws.shape[0] < M or ws.shape[1] < N + (kpad if adapter is not None else 0) or n != M:
+    if ws.dtype is not F32 or ws.dim() != 2 or ws.shape[0] < M or ws.shape[1] < N + (kpad if adapter is not None else 0) or n != M:
         raise ValueError(f"ws must be fp32 [>= {M}, >= {N} and the low-rank columns], and q_out have {M} rows")
     dev = _device(ws, pos, slot, k_cache, v_cache, k_scale, v_scale, q_out)
     ptr = lambda t: 0 if t is None else t.data_ptr()      # noqa: E731
     _launch(dev, "artb_decode_finalize_qkv_q8", ws.data_ptr(), ws.stride(0), M, Hq, Hkv, hd, kpad, ptr(bias), ptr(adapter), ptr(B_all),
             B_all.stride(0) if B_all is not None else 0, cols, pos.data_ptr(), theta, ptr(q_norm), ptr(k_norm), eps, slot.data_ptr(),
-            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, kind, q_out.data_ptr(), ldq, nb)
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, kind, to, ldq, nb)
 
 
 def finalize_covers(Hq: int, Hkv: int) -> bool:
@@ -181,15 +187,17 @@ def kv_rows_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
                dst: torch.Tensor, k_col: int, v_col: int) -> None:
     """The cached keys and values at ``slot`` (int32 [n]) as bf16 into the k and v columns of ``dst[:n]``; zeros where negative."""
     nb, hkv, bs, hd, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
-    have, ld = _rows("dst", dst, k_col, v_col, hkv * hd)
+    have, ld, to = _rows("dst", dst, k_col, v_col, hkv * hd)
     if abs(k_col - v_col) < hkv * hd or ld < max(k_col, v_col) + hkv * hd:
         raise ValueError("the columns of keys and values, or the rows of dst, overlap")
     n = slot.numel()
     _index("slot", slot, n)
     if n > have:
         raise ValueError(f"{n} slots for {have} rows")
-    dev = _device(dst, slot, k_cache, v_cache, k_scale, v_scale)
-    _launch(dev, "artb_kv_rows_q8", dst.data_ptr(), slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+    dev = dst.get_device()
+    if not (0 <= dev == slot.get_device() == k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device()):
+        _device(dst, slot, k_cache, v_cache, k_scale, v_scale)
+    _launch(dev, "artb_kv_rows_q8", to, slot.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), nb, n, ld, k_col, v_col, hkv, hd, bs, kind)
 
 
@@ -224,16 +232,18 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
     if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > 16 * Hkv:
         raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
-    n, ldq = _rows("q", q, 0, 0, Hq * hd)
-    m, ldo = _rows("out", out, 0, 0, Hq * hd)
-    at, to = q.data_ptr(), out.data_ptr()
+    n, ldq, at = _rows("q", q, 0, 0, Hq * hd)
+    m, ldo, to = _rows("out", out, 0, 0, Hq * hd)
     if m != n or ldo < Hq * hd or (abs(to - at) < 2 * n * max(ldq, ldo) and _meet(at, ldq, to, ldo, n, Hq * hd)):
         raise ValueError(f"out must have {n} rows that do not overlap, nor lie where q does")
     _index("ctx_len", ctx_len, n)
     table = block_table.shape
-    if block_table.dtype is not torch.int32 or len(table) != 2 or table[0] != n or table[1] < 1 or not block_table.is_contiguous():
+    if block_table.dtype is not I32 or len(table) != 2 or table[0] != n or table[1] < 1 or not block_table.is_contiguous():
         raise ValueError(f"block_table must be contiguous int32 [{n}, width]")
-    dev = _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
+    dev = q.get_device()
+    if not (0 <= dev == k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device()
+            == block_table.get_device() == ctx_len.get_device() == out.get_device() == ws.get_device()):
+        _device(q, k_cache, v_cache, k_scale, v_scale, block_table, ctx_len, out, ws)
     if n and (ws.nbytes < _decode_bytes(n, Hq, Hkv, hd, dev) or not ws.is_contiguous()):
         raise ValueError(f"workspace of {ws.nbytes} bytes, {_decode_bytes(n, Hq, Hkv, hd, dev)} needed in a row")
     _launch(dev, "artb_paged_decode_q8", at, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
