@@ -169,9 +169,20 @@ def decode_finalize_qkv_q8(ws: torch.Tensor, M: int, Hq: int, Hkv: int, hd: int,
     _index("pos", pos, M)
     n, ldq, to = _rows("q_out", q_out, 0, 0, Hq * hd)
     N = (Hq + 2 * Hkv) * hd
-    if ws.dtype is not F32 or ws.dim() != 2 or ws.shape[0] < M or ws.shape[1] < N + (kpad if adapter is not None else 0) or n != M:
+    if (ws.dtype is not F32 or ws.dim() != 2 or ws.shape[0] < M or ws.shape[1] < N + (kpad if adapter is not None else 0) or ws.stride(1) != 1
+            or n != M):
         raise ValueError(f"ws must be fp32 [>= {M}, >= {N} and the low-rank columns], and q_out have {M} rows")
-    dev = _device(ws, pos, slot, k_cache, v_cache, k_scale, v_scale, q_out)
+    given = []
+    for name, t, dtype, size in (("bias", bias, F32, N), ("adapter", adapter, I32, M), ("q_norm", q_norm, BF16, hd), ("k_norm", k_norm, BF16, hd)):
+        if t is not None:
+            if t.dtype is not dtype or t.numel() < size or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dtype} of {size} numbers")
+            given.append(t)
+    if adapter is not None:
+        if B_all is None or B_all.dtype is not BF16 or B_all.dim() != 2 or B_all.shape[1] < N or B_all.stride(1) != 1:
+            raise ValueError(f"B_all must be bf16 [rows of all adapters, >= {N}]")
+        given.append(B_all)
+    dev = _device(ws, pos, slot, k_cache, v_cache, k_scale, v_scale, q_out, *given)
     ptr = lambda t: 0 if t is None else t.data_ptr()      # noqa: E731
     _launch(dev, "artb_decode_finalize_qkv_q8", ws.data_ptr(), ws.stride(0), M, Hq, Hkv, hd, kpad, ptr(bias), ptr(adapter), ptr(B_all),
             B_all.stride(0) if B_all is not None else 0, cols, pos.data_ptr(), theta, ptr(q_norm), ptr(k_norm), eps, slot.data_ptr(),

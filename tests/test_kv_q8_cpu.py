@@ -105,10 +105,10 @@ def test_decode(kw, says):
         decode(cache(), **kw)
 
 
-def finish(c, M=3, heads=(4, 2, 64), pos=None, slot=None, q=None, ws=None):
+def finish(c, M=3, heads=(4, 2, 64), pos=None, slot=None, q=None, ws=None, **kw):
     z = lambda *s: torch.zeros(*s, dtype=torch.int32)         # noqa: E731
     kv_q8.decode_finalize_qkv_q8(torch.zeros(4, 512) if ws is None else ws, M, *heads, 0, z(3) if pos is None else pos, 1e6, z(3) if slot is None else slot,
-                                 *c, torch.zeros(3, 256, dtype=BF) if q is None else q)
+                                 *c, torch.zeros(3, 256, dtype=BF) if q is None else q, **kw)
 
 
 @pytest.mark.parametrize("kw,says", [
@@ -121,6 +121,15 @@ def finish(c, M=3, heads=(4, 2, 64), pos=None, slot=None, q=None, ws=None):
     (dict(ws=torch.zeros(2, 512)), "ws must be"),
     (dict(ws=torch.zeros(4, 504)), "ws must be"),
     (dict(ws=torch.zeros(4, 512, dtype=BF)), "ws must be"),
+    (dict(ws=torch.zeros(512, 4).t()), "ws must be"),
+    (dict(bias=torch.zeros(512, dtype=BF)), "bias must be"),
+    (dict(bias=torch.zeros(511)), "bias must be"),
+    (dict(q_norm=torch.zeros(64), k_norm=torch.zeros(64, dtype=BF)), "q_norm must be"),
+    (dict(q_norm=torch.zeros(64, dtype=BF), k_norm=torch.zeros(128, dtype=BF)[::2]), "k_norm must be"),
+    (dict(adapter=torch.zeros(2, dtype=torch.int32)), "adapter must be"),
+    (dict(adapter=torch.zeros(3, dtype=torch.int32)), "B_all must be"),
+    (dict(adapter=torch.zeros(3, dtype=torch.int32), B_all=torch.zeros(8, 504, dtype=BF)), "B_all must be"),
+    (dict(adapter=torch.zeros(3, dtype=torch.int32), B_all=torch.zeros(8, 512)), "B_all must be"),
     (dict(), "one CUDA device"),
 ])
 def test_finish(kw, says):
