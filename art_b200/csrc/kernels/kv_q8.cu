@@ -20,74 +20,121 @@ namespace artb {
 
 // A run is a stretch of neighbouring rows whose slots are neighbours in one block.  A warp takes a run's part for one kv head, of
 // keys or of values: it looks for the runs that begin among its ROWS rows and follows them to their ends.  A lane holds 8 values
-// of a row, HD / 8 lanes to a row, ITERS * 32 * 8 / HD rows at a time in registers; longer runs are read twice.  FULL: the rows
-// are a multiple of that.
-template <int KIND, int HD, int ITERS, bool FULL>
-__device__ __forceinline__ void kw_run(const __nv_bfloat16* x, int ld, int n, int at, int block_size, uint8_t* codes, float* sp) {
-  constexpr int LPR = HD / 8, RPI = 32 / LPR, BATCH = ITERS * RPI;
-  const int lane = threadIdx.x & 31, sub = lane / LPR, c = (lane % LPR) * 8;
-  const float held = __ldcg(sp);
-  uint4 raw[ITERS];
-  auto load = [&](int first) {
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
-      const int r = first + i * RPI + sub;
-      raw[i] = FULL || r < n ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(r) * ld + c) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  // largest |value|: the bits of bf16 magnitudes order like integers, two at a time
+// of a row, HD / 8 lanes to a row: of up to 16 rows in registers, of longer runs in its own places of shared memory, where 32 rows
+// are under way at a time; runs longer than that are read twice.  (14,000 rows in blocks of 32: 19.0 us, 20.4 with 16 rows of 32 in
+// registers at a time.  Shared memory for runs of 16 too takes 12.6 us where registers take 11.8: 14,760 rows in blocks of 16.)
+template <int KIND, int HD>
+struct KwRun {
+  static constexpr int LPR = HD / 8, RPI = 32 / LPR, STEP = 16 / RPI;     // pieces of a lane per 16 rows
+  static constexpr int FIT = 32;
+  static constexpr int ROOM = FIT * LPR;                                  // 16-byte places of a warp
+
+  const __nv_bfloat16* x;      // of the first row
+  int ld, n, at, block_size;   // rows, the first one's place in the block
+  uint8_t* codes;              // of the block
+  float* sp;
   uint32_t top = 0;
-  for (int first = 0; first < n; first += BATCH) {
-    load(first);
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
-      top = __vmaxu2(top, raw[i].x & 0x7fff7fffu);
-      top = __vmaxu2(top, raw[i].y & 0x7fff7fffu);
-      top = __vmaxu2(top, raw[i].z & 0x7fff7fffu);
-      top = __vmaxu2(top, raw[i].w & 0x7fff7fffu);
-    }
+  float inv;
+
+  static __device__ __forceinline__ int sub() { return (threadIdx.x & 31) / LPR; }
+  static __device__ __forceinline__ int col() { return (threadIdx.x & 31) % LPR * 8; }
+
+  // largest |value|: the bits of bf16 magnitudes order like integers, two at a time
+  __device__ __forceinline__ void look(const uint4& v) {
+    top = __vmaxu2(top, v.x & 0x7fff7fffu);
+    top = __vmaxu2(top, v.y & 0x7fff7fffu);
+    top = __vmaxu2(top, v.z & 0x7fff7fffu);
+    top = __vmaxu2(top, v.w & 0x7fff7fffu);
   }
-  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-  const Q8Scale scale = q8_new_scale<KIND>(top, held, at == 0);
-  const float inv = scale.inv;
-  const bool bad = isnan(inv);
-  __syncwarp();                              // every lane has the old scale
-  if (lane == 0) *sp = scale.to;
-  if (scale.down != 1.f) {
-    for (int v = lane; v < block_size * (HD / 16); v += 32) {
-      if (v / (HD / 16) >= at && v / (HD / 16) < at + n) continue;
-      uint4* p = reinterpret_cast<uint4*>(codes) + v;
-      *p = q8_lower<KIND>(*p, scale.down);
-    }
-  }
-  for (int first = 0; first < n; first += BATCH) {
-    if (n > BATCH) load(first);              // else the only batch is still in registers
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
-      const int r = first + i * RPI + sub;
-      if (!FULL && r >= n) continue;
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[2 * j] = __uint_as_float(w[j] << 16) * inv;
-        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
+
+  __device__ __forceinline__ void rescale(float held) {
+    const int lane = threadIdx.x & 31;
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    const Q8Scale scale = q8_new_scale<KIND>(top, held, at == 0);
+    inv = scale.inv;
+    __syncwarp();                              // every lane has the old scale
+    if (lane == 0) *sp = scale.to;
+    if (scale.down != 1.f) {
+      for (int v = lane; v < block_size * (HD / 16); v += 32) {
+        if (v / (HD / 16) >= at && v / (HD / 16) < at + n) continue;
+        uint4* p = reinterpret_cast<uint4*>(codes) + v;
+        *p = q8_lower<KIND>(*p, scale.down);
       }
-      uint2 out = make_uint2(q8_encode4<KIND>(f[0], f[1], f[2], f[3]), q8_encode4<KIND>(f[4], f[5], f[6], f[7]));
-      if (bad) out = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>(codes + static_cast<size_t>(at + r) * HD + c) = out;
     }
   }
-}
+
+  __device__ __forceinline__ void put(const uint4& v, int row) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[2 * j] = __uint_as_float(w[j] << 16) * inv;
+      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
+    }
+    uint2 out = make_uint2(q8_encode4<KIND>(f[0], f[1], f[2], f[3]), q8_encode4<KIND>(f[4], f[5], f[6], f[7]));
+    if (isnan(inv)) out = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(codes + static_cast<size_t>(at + row) * HD + col()) = out;
+  }
+
+  // up to ITERS * RPI rows; FULL: as many
+  template <int ITERS, bool FULL>
+  __device__ __forceinline__ void held() {
+    const float before = __ldcg(sp);
+    uint4 raw[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+      const int r = i * RPI + sub();
+      raw[i] = FULL || r < n ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(r) * ld + col()) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) look(raw[i]);
+    rescale(before);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+      if (FULL || i * RPI + sub() < n) put(raw[i], i * RPI + sub());
+  }
+
+  template <class F>
+  __device__ __forceinline__ void pieces(int rows, F f) const {           // of this lane: the place in `room`, the row
+#pragma unroll 1
+    for (int b = 0; b < rows; b += 16) {
+#pragma unroll
+      for (int i = 0; i < STEP; ++i)
+        if (b + i * RPI + sub() < rows) f(b * LPR + i * 32 + static_cast<int>(threadIdx.x & 31), b + i * RPI + sub());
+    }
+  }
+
+  __device__ __forceinline__ void staged(uint4* room) {
+    const float before = __ldcg(sp);
+    auto bring = [&](int first, int rows) {
+      pieces(rows, [&](int place, int r) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(room + place)),
+                     "l"(x + static_cast<size_t>(first + r) * ld + col())
+                     : "memory");
+      });
+      asm volatile("cp.async.wait_all;" ::: "memory");                    // a lane reads what it brought itself
+    };
+    for (int first = 0; first < n; first += FIT) {
+      bring(first, min(FIT, n - first));
+      pieces(min(FIT, n - first), [&](int place, int) { look(room[place]); });
+    }
+    rescale(before);
+    for (int first = 0; first < n; first += FIT) {
+      if (n > FIT) bring(first, min(FIT, n - first));
+      pieces(min(FIT, n - first), [&](int place, int r) { put(room[place], first + r); });
+    }
+  }
+};
 
 // ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 3.3 us, 4.6 with four to a warp, 12 with
-// sixteen), a block's worth where prompts bring many (14,000 rows: 20 us, 26 with four to a warp, 64 with one).
+// sixteen), a block's worth where prompts bring many (14,000 rows, when that was 20 us: 26 with four to a warp, 64 with one).
 template <int KIND, int HD, int ROWS>
 __global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 6)
 kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int v_col, const int* __restrict__ slot,
                    uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int M, int Hkv, int block_size,
                    int block_shift, long num_blocks, int* status) {
   static_assert(ROWS <= 16, "a warp sees 32 rows at once, and a run of 16 to its end");
+  extern __shared__ uint4 kw_room[];           // where blocks have more than 16 rows
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, part = blockIdx.y * 4 + (threadIdx.x >> 5), row0 = blockIdx.x * ROWS;
@@ -120,15 +167,11 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
       if (more != 0xffffffffu) break;
     }
     const long head = static_cast<long>(block) * Hkv + h;
-    uint8_t* codes = cache + head * block_size * HD;
-    const __nv_bfloat16* rows = x + static_cast<size_t>(r0) * ld;
-    if (n * (HD / 8) <= 32) {
-      kw_run<KIND, HD, 1, false>(rows, ld, n, at, block_size, codes, scales + head);
-    } else if (n % 16 == 0) {                // whole blocks, for the most part
-      kw_run<KIND, HD, HD / 16, true>(rows, ld, n, at, block_size, codes, scales + head);
-    } else {
-      kw_run<KIND, HD, HD / 16, false>(rows, ld, n, at, block_size, codes, scales + head);
-    }
+    KwRun<KIND, HD> run{x + static_cast<size_t>(r0) * ld, ld, n, at, block_size, cache + head * block_size * HD, scales + head};
+    if (n * (HD / 8) <= 32) run.template held<1, false>();
+    else if (n > 16) run.staged(kw_room + (threadIdx.x >> 5) * KwRun<KIND, HD>::ROOM);
+    else if (n == 16) run.template held<HD / 16, true>();                 // whole blocks, for the most part
+    else run.template held<HD / 16, false>();
   }
 }
 
@@ -207,7 +250,8 @@ ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
 #define ARTB_KW(KIND_, HD_)                                                                                                  \
   if (kind == KIND_ && hd == HD_) {                                                                                          \
     auto go = [&](auto kern, int rows) {                                                                                     \
-      return static_cast<int>(launch_ahead(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), 0, st,          \
+      const int room = block_size > 16 ? 4 * KwRun<KIND_, HD_>::ROOM * 16 : 0;                                               \
+      return static_cast<int>(launch_ahead(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), room, st,       \
                                             (const __nv_bfloat16*)a->rows, ld, a->k_col, a->v_col, a->slot,                  \
                                             (uint8_t*)a->k_cache, (uint8_t*)a->v_cache, a->k_scale, a->v_scale, M, Hkv,      \
                                             block_size, shift, a->num_blocks, a->status));                                   \
