@@ -21,8 +21,8 @@ namespace artb {
 // A run is a stretch of neighbouring rows whose slots are neighbours in one block.  A warp takes a run's part for one kv head, of
 // keys or of values: it looks for the runs that begin among its ROWS rows and follows them to their ends.  A lane holds 8 values
 // of a row, HD / 8 lanes to a row: of up to 16 rows in registers, of longer runs in its own places of shared memory, where 32 rows
-// are under way at a time; runs longer than that are read twice.  (14,000 rows in blocks of 32: 19.0 us, 20.4 with 16 rows of 32 in
-// registers at a time.  Shared memory for runs of 16 too takes 12.6 us where registers take 11.8: 14,760 rows in blocks of 16.)
+// are under way at a time; runs longer than that are read twice.  (14,000 rows in blocks of 32: 17.7 us, 19.1 with 16 rows of 32 in
+// registers at a time.  Shared memory for runs of 16 too takes 0.8 us more than registers, of 11.8: 14,760 rows in blocks of 16.)
 template <int KIND, int HD>
 struct KwRun {
   static constexpr int LPR = HD / 8, RPI = 32 / LPR, STEP = 16 / RPI;     // pieces of a lane per 16 rows
@@ -129,7 +129,7 @@ struct KwRun {
 // ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 3.3 us, 4.6 with four to a warp, 12 with
 // sixteen), a block's worth where prompts bring many (14,000 rows, when that was 20 us: 26 with four to a warp, 64 with one).
 template <int KIND, int HD, int ROWS>
-__global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 6)
+__global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 7)
 kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int v_col, const int* __restrict__ slot,
                    uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int M, int Hkv, int block_size,
                    int block_shift, long num_blocks, int* status) {
@@ -145,6 +145,12 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
   uint8_t* cache = is_v ? v_cache : k_cache;
   float* scales = is_v ? v_scale : k_scale;
 
+  if (ROWS == 16) {            // the rows are on their way to L2 while the slots are looked up: 10.6 us instead of 11.5 (14,760 rows);
+                               // calls of fewer rows, which are in L2 already more often than not, lose 0.2 us by it
+    constexpr int LINES = HD / 64 ? HD / 64 : 1;
+    if (lane < ROWS * LINES && row0 + lane / LINES < M)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(x + static_cast<size_t>(row0 + lane / LINES) * ld + lane % LINES * 64));
+  }
   const int s = row0 + lane < M ? slot[row0 + lane] : -1;
   int prev = __shfl_up_sync(0xffffffffu, s, 1);
   if (lane == 0) prev = row0 > 0 ? slot[row0 - 1] : -1;
