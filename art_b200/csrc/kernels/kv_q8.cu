@@ -23,11 +23,11 @@ namespace artb {
 // of a row, HD / 8 lanes to a row: of up to 16 rows in registers, of longer runs in its own places of shared memory, where 32 rows
 // are under way at a time; runs longer than that are read twice.  (14,000 rows in blocks of 32: 17.7 us, 19.1 with 16 rows of 32 in
 // registers at a time.  Shared memory for runs of 16 too takes 0.8 us more than registers, of 11.8: 14,760 rows in blocks of 16.)
+constexpr int KW_FIT = 32;
 template <int KIND, int HD>
 struct KwRun {
   static constexpr int LPR = HD / 8, RPI = 32 / LPR, STEP = 16 / RPI;     // pieces of a lane per 16 rows
-  static constexpr int FIT = 32;
-  static constexpr int ROOM = FIT * LPR;                                  // 16-byte places of a warp
+  static constexpr int PLACE = LPR * 16;                                  // bytes of a row
 
   const __nv_bfloat16* x;      // of the first row
   int ld, n, at, block_size;   // rows, the first one's place in the block
@@ -47,15 +47,24 @@ struct KwRun {
     top = __vmaxu2(top, v.w & 0x7fff7fffu);
   }
 
-  __device__ __forceinline__ void rescale(float held) {
-    const int lane = threadIdx.x & 31;
+  // The block's new scale from the one that all have read before; `tops`: a place for each of TEAM warps that share the run.
+  template <int TEAM>
+  __device__ __forceinline__ void rescale(float held, uint32_t* tops) {
+    const int thread = TEAM > 1 ? threadIdx.x : threadIdx.x & 31;
     top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    if (TEAM > 1) {
+      if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) top = max(top, tops[w]);
+    } else {
+      __syncwarp();
+    }
     const Q8Scale scale = q8_new_scale<KIND>(top, held, at == 0);
     inv = scale.inv;
-    __syncwarp();                              // every lane has the old scale
-    if (lane == 0) *sp = scale.to;
+    if (thread == 0) *sp = scale.to;
     if (scale.down != 1.f) {
-      for (int v = lane; v < block_size * (HD / 16); v += 32) {
+      for (int v = thread; v < block_size * (HD / 16); v += TEAM * 32) {
         if (v / (HD / 16) >= at && v / (HD / 16) < at + n) continue;
         uint4* p = reinterpret_cast<uint4*>(codes) + v;
         *p = q8_lower<KIND>(*p, scale.down);
@@ -76,22 +85,22 @@ struct KwRun {
     *reinterpret_cast<uint2*>(codes + static_cast<size_t>(at + row) * HD + col()) = out;
   }
 
-  // up to ITERS * RPI rows; FULL: as many
-  template <int ITERS, bool FULL>
-  __device__ __forceinline__ void held() {
+  // Up to ITERS * RPI rows from `lo` on, of each of TEAM warps; FULL: as many.
+  template <int ITERS, bool FULL, int TEAM = 1>
+  __device__ __forceinline__ void held(uint32_t* tops = nullptr, int lo = 0) {
     const float before = __ldcg(sp);
     uint4 raw[ITERS];
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
-      const int r = i * RPI + sub();
+      const int r = lo + i * RPI + sub();
       raw[i] = FULL || r < n ? *reinterpret_cast<const uint4*>(x + static_cast<size_t>(r) * ld + col()) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) look(raw[i]);
-    rescale(before);
+    rescale<TEAM>(before, tops);
 #pragma unroll
     for (int i = 0; i < ITERS; ++i)
-      if (FULL || i * RPI + sub() < n) put(raw[i], i * RPI + sub());
+      if (FULL || lo + i * RPI + sub() < n) put(raw[i], lo + i * RPI + sub());
   }
 
   template <class F>
@@ -104,8 +113,13 @@ struct KwRun {
     }
   }
 
-  __device__ __forceinline__ void staged(uint4* room) {
+  // TEAM warps share the rows, FIT of them each in `room` at a time
+  template <int TEAM, int FIT>
+  __device__ __forceinline__ void staged(uint4* room, uint32_t* tops) {
     const float before = __ldcg(sp);
+    const int share = TEAM > 1 ? (n + 16 * TEAM - 1) / (16 * TEAM) * 16 : n;
+    if (TEAM > 1 && share == 16) return held<STEP, false, TEAM>(tops, (threadIdx.x >> 5) * 16);
+    const int lo = TEAM > 1 ? static_cast<int>(threadIdx.x >> 5) * share : 0, hi = min(n, lo + share);
     auto bring = [&](int first, int rows) {
       pieces(rows, [&](int place, int r) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(room + place)),
@@ -114,30 +128,34 @@ struct KwRun {
       });
       asm volatile("cp.async.wait_all;" ::: "memory");                    // a lane reads what it brought itself
     };
-    for (int first = 0; first < n; first += FIT) {
-      bring(first, min(FIT, n - first));
-      pieces(min(FIT, n - first), [&](int place, int) { look(room[place]); });
+    for (int first = lo; first < hi; first += FIT) {
+      bring(first, min(FIT, hi - first));
+      pieces(min(FIT, hi - first), [&](int place, int) { look(room[place]); });
     }
-    rescale(before);
-    for (int first = 0; first < n; first += FIT) {
-      if (n > FIT) bring(first, min(FIT, n - first));
-      pieces(min(FIT, n - first), [&](int place, int r) { put(room[place], first + r); });
+    rescale<TEAM>(before, tops);
+    for (int first = lo; first < hi; first += FIT) {
+      if (hi - lo > FIT) bring(first, min(FIT, hi - first));
+      pieces(min(FIT, hi - first), [&](int place, int r) { put(room[place], first + r); });
     }
   }
 };
 
 // ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 3.3 us, 4.6 with four to a warp, 12 with
 // sixteen), a block's worth where prompts bring many (14,000 rows, when that was 20 us: 26 with four to a warp, 64 with one).
-template <int KIND, int HD, int ROWS>
+// TEAM: of blocks of more than 32 rows a run is four warps', which find the same runs and share the rows of a long one (1000 rows in
+// blocks of 64: 4.5 us, 8.1 with a warp to each; 8192 in blocks of 128: 17.7 and 23.6; but 512 rows in as many blocks 6.3 and 5.2, and
+// 2000 rows in blocks of 32 7.6 and 6.9).
+template <int KIND, int HD, int ROWS, int TEAM>
 __global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 7)
 kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int v_col, const int* __restrict__ slot,
                    uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int M, int Hkv, int block_size,
                    int block_shift, long num_blocks, int* status) {
   static_assert(ROWS <= 16, "a warp sees 32 rows at once, and a run of 16 to its end");
   extern __shared__ uint4 kw_room[];           // where blocks have more than 16 rows
+  __shared__ uint32_t s_top[4];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, part = blockIdx.y * 4 + (threadIdx.x >> 5), row0 = blockIdx.x * ROWS;
+  const int lane = threadIdx.x & 31, part = TEAM > 1 ? blockIdx.y : blockIdx.y * 4 + (threadIdx.x >> 5), row0 = blockIdx.x * ROWS;
   if (part >= 2 * Hkv) return;
   const bool is_v = part >= Hkv;
   const int h = is_v ? part - Hkv : part;
@@ -148,7 +166,7 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
   if (ROWS == 16) {            // the rows are on their way to L2 while the slots are looked up: 10.6 us instead of 11.5 (14,760 rows);
                                // calls of fewer rows, which are in L2 already more often than not, lose 0.2 us by it
     constexpr int LINES = HD / 64 ? HD / 64 : 1;
-    if (lane < ROWS * LINES && row0 + lane / LINES < M)
+    if ((TEAM == 1 || threadIdx.x < 32) && lane < ROWS * LINES && row0 + lane / LINES < M)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(x + static_cast<size_t>(row0 + lane / LINES) * ld + lane % LINES * 64));
   }
   const int s = row0 + lane < M ? slot[row0 + lane] : -1;
@@ -160,7 +178,9 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
   // a second run in the block of the row before would be a second warp's at the same scale: refused
   const bool astray = s >= 0 && !goes_on && prev >= blk * block_size && prev - blk * block_size < block_size;
   if (astray && lane < ROWS && status) atomicMax(status, ST_BAD_ARGS);
-  for (uint32_t todo = __ballot_sync(0xffffffffu, lane < ROWS && s >= 0 && !goes_on && !astray); todo; todo &= todo - 1) {
+  // of a team, a run of 17 rows or more is all warps', one of fewer is one warp's
+  const bool whose = TEAM == 1 || (lane & 3) == static_cast<int>(threadIdx.x >> 5) || (on >> lane >> 1 & 0xffffu) == 0xffffu;
+  for (uint32_t todo = __ballot_sync(0xffffffffu, lane < ROWS && s >= 0 && !goes_on && !astray && whose); todo; todo &= todo - 1) {
     const int i = __ffs(todo) - 1, s0 = __shfl_sync(0xffffffffu, s, i), block = __shfl_sync(0xffffffffu, blk, i);
     if (!q8_index_ok(s0, num_blocks * block_size, status)) continue;
     const int r0 = row0 + i, at = s0 - block * block_size;
@@ -174,8 +194,9 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
     }
     const long head = static_cast<long>(block) * Hkv + h;
     KwRun<KIND, HD> run{x + static_cast<size_t>(r0) * ld, ld, n, at, block_size, cache + head * block_size * HD, scales + head};
-    if (n * (HD / 8) <= 32) run.template held<1, false>();
-    else if (n > 16) run.staged(kw_room + (threadIdx.x >> 5) * KwRun<KIND, HD>::ROOM);
+    uint4* room = kw_room + (threadIdx.x >> 5) * KW_FIT * KwRun<KIND, HD>::LPR;
+    if (n > 16) run.template staged<TEAM, KW_FIT>(room, s_top);           // one at most begins among 16 rows
+    else if (n * (HD / 8) <= 32) run.template held<1, false>();
     else if (n == 16) run.template held<HD / 16, true>();                 // whole blocks, for the most part
     else run.template held<HD / 16, false>();
   }
@@ -255,16 +276,17 @@ ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
   const int shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctz(block_size);
 #define ARTB_KW(KIND_, HD_)                                                                                                  \
   if (kind == KIND_ && hd == HD_) {                                                                                          \
-    auto go = [&](auto kern, int rows) {                                                                                     \
-      const int room = block_size > 16 ? 4 * KwRun<KIND_, HD_>::ROOM * 16 : 0;                                               \
-      return static_cast<int>(launch_ahead(kern, dim3((M + rows - 1) / rows, (2 * Hkv + 3) / 4), dim3(128), room, st,       \
+    auto go = [&](auto kern, int rows, int parts) {                                                                          \
+      const int room = block_size > 16 ? 4 * KW_FIT * KwRun<KIND_, HD_>::PLACE : 0;                                          \
+      return static_cast<int>(launch_ahead(kern, dim3((M + rows - 1) / rows, (2 * Hkv + parts - 1) / parts), dim3(128), room, st, \
                                             (const __nv_bfloat16*)a->rows, ld, a->k_col, a->v_col, a->slot,                  \
                                             (uint8_t*)a->k_cache, (uint8_t*)a->v_cache, a->k_scale, a->v_scale, M, Hkv,      \
                                             block_size, shift, a->num_blocks, a->status));                                   \
     };                                                                                                                       \
-    if (M <= 256) return go(kv_write_q8_kernel<KIND_, HD_, 1>, 1);                                                           \
-    if (M <= 2048) return go(kv_write_q8_kernel<KIND_, HD_, 4>, 4);                                                          \
-    return go(kv_write_q8_kernel<KIND_, HD_, 16>, 16);                                                                       \
+    if (M <= 256) return go(kv_write_q8_kernel<KIND_, HD_, 1, 1>, 1, 4);                                                     \
+    if (block_size > 32) return go(kv_write_q8_kernel<KIND_, HD_, 16, 4>, 16, 1);                                            \
+    if (M <= 2048) return go(kv_write_q8_kernel<KIND_, HD_, 4, 1>, 4, 4);                                                    \
+    return go(kv_write_q8_kernel<KIND_, HD_, 16, 1>, 16, 4);                                                                 \
   }
   ARTB_KW(Q8_E4M3, 128) ARTB_KW(Q8_E4M3, 64) ARTB_KW(Q8_E4M3, 32)
   ARTB_KW(Q8_INT8, 128) ARTB_KW(Q8_INT8, 64) ARTB_KW(Q8_INT8, 32)

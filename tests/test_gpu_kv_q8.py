@@ -1,4 +1,6 @@
 """A paged cache in 8 bits on the GPU: writes, read-back and decode attention against their definitions in 64 bits."""
+import random
+
 import pytest
 import torch
 
@@ -93,6 +95,47 @@ def test_writes_of_a_batch(dtype):
     same(cache, *o)
     assert not torch.equal(cache[0].double(), before[0].double())
     assert torch.equal(cache[0][36:].double(), before[0][36:].double())        # blocks that no row names
+
+
+@KINDS
+@pytest.mark.parametrize("kv,hd,bs", [(2, 128, 48), (3, 64, 64), (1, 32, 128), (2, 128, 160), (2, 64, 32), (1, 128, 32)])
+@pytest.mark.parametrize("many", [False, True])
+def test_writes_of_long_runs(dtype, kv, hd, bs, many):
+    """More rows than a step has, into long blocks: runs of every length beside one another, from any place of a block on, that begin
+    at any row of the call, rows that are not written between them, and a second call that goes on in the same blocks with values
+    that raise the scales of some."""
+    g = torch.Generator(device=DEV).manual_seed(kv * hd + bs)
+    r = random.Random(bs + hd)
+    lens = [1, 2, 15, 16, 17, 18, 31, 32, 33, 47, 48, 49, 63, 64, 65, 1, 1, 1, 96, 127, 128, 129, 160]
+    lens = [min(n, bs) for n in lens] + ([bs] * (2300 // bs) if many else [])
+    r.shuffle(lens)
+    nb = len(lens) + 2
+    cache = empty(nb, kv, bs, hd, dtype)
+    o = oracles_of(cache)
+    full = keys(nb * bs, kv, hd, g, spread=0.2)
+    write(full, 0, list(range(nb * bs)), cache, o, kv, hd)
+    for size in (0.02, 1.0, 40.0):
+        slots, blocks = [], list(range(len(lens)))
+        r.shuffle(blocks)
+        for b, n in zip(blocks, lens):
+            at = r.choice([0, bs - n, r.randint(0, bs - n)])
+            slots += [-1] * r.choice([0, 0, 1, 3]) + [b * bs + at + i for i in range(n)]
+        assert len(slots) > (2048 if many else 256)
+        write((keys(len(slots), kv, hd, g, extra=8).float() * size).bfloat16(), 8, slots, cache, o, kv, hd)
+        same(cache, *o)
+
+
+@KINDS
+def test_a_step_into_long_blocks(dtype):
+    """A token each of more sequences than a warp per row is for."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    kv, hd, bs, n = 2, 64, 64, 301
+    cache = empty(n + 2, kv, bs, hd, dtype)
+    o = oracles_of(cache)
+    write(keys((n + 2) * bs, kv, hd, g, spread=0.2), 0, list(range((n + 2) * bs)), cache, o, kv, hd)
+    step = [b * bs + (7 * b) % bs for b in range(n)]
+    write(keys(n, kv, hd, g), 0, step, cache, o, kv, hd)
+    same(cache, *o)
 
 
 @KINDS
