@@ -285,7 +285,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int NT = HEADS / 8, JT = HD / 16, KW = HD / 16, VW = HD / 32, STAGES = pq_stages(HD, HEADS);
   extern __shared__ uint8_t pq_smem_raw[];
   uint8_t* rings = pq_smem_raw + (1024 - (smem_u32(pq_smem_raw) & 1023));
-  __shared__ int s_warp[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES];
+  __shared__ int s_warp[PQ_WARPS], s_longest[PQ_WARPS], s_first[PQ_ENTRIES], s_len[PQ_ENTRIES];
   __shared__ volatile int s_abort;
   __shared__ int s_goes_on[PQ_WARPS];       // how a warp goes on with the sequence that the one before it ends in (PqGoesOn)
   __shared__ int4 s_part[2];                // sequences that the CTA is the last to finish a part of: number, first share, parts, 1
@@ -324,7 +324,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll 1
     for (int d = 0; d < G * HD / 8; ++d) o[d] = make_uint4(0, 0, 0, 0);
   };
-  int own = 0;
+  int own = 0, longest = 0;
   if (run == 1) {
     int len[PQ_ENTRIES / PQ_THREADS];                  // all lengths on their way at once
 #pragma unroll
@@ -344,6 +344,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     s_first[e] = own;
     if (run == 1) {
       own += tiles_in(s_len[e]);
+      longest = max(longest, tiles_in(s_len[e]));
     } else {
 #pragma unroll 1
       for (int i = e * run; i < min(nseq, (e + 1) * run); ++i) {
@@ -359,17 +360,27 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_warp[warp] = incl;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) {
+    s_warp[warp] = incl;
+    s_longest[warp] = longest;
+  }
   __syncthreads();
   int total = 0, before = incl - own;
 #pragma unroll
   for (int w = 0; w < PQ_WARPS; ++w) {
     if (w < warp) before += s_warp[w];
     total += s_warp[w];
+    longest = max(longest, s_longest[w]);
   }
 #pragma unroll 1
   for (int e = e0; e < e1; ++e) s_first[e] += before;
-  const int per = max(PQ_MIN_TILES, static_cast<int>(__umulhi(total + shares - 1, per_share)) + (shares == 1)), per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
+  // The parts of a sequence are added up by one CTA.  With t microseconds for a warp's tile and p for a part of L tiles, shares of n
+  // cost n / 4 t + L / n p, the least at n = 2 sqrt(L p / t); p goes with the part's size.  One context of 16,000 keys, 8 heads of 128
+  // to a kv head: 12.6 us, 16.6 with shares as small as the chip has room for; 16 heads: 18.5 and 26.9.
+  const int few = static_cast<int>(sqrtf(0.3f * HEADS * HD / 1024 * longest));
+  const int per = max(max(PQ_MIN_TILES, few), static_cast<int>(__umulhi(total + shares - 1, per_share)) + (shares == 1));
+  const int per_warp = (per + PQ_WARPS - 1) / PQ_WARPS;
   const int at = share * per;
   if (at >= total) return;                  // the whole CTA
   const int end = min(total, at + per);
