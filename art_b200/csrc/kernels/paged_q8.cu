@@ -17,7 +17,7 @@
 // Bound by the cache's bytes, and beside them by what a launch begins and ends with.  256 contexts of 512 to 2032 keys, 28 / 4 heads
 // of 128, e4m3 (338 MB, 52 us at the copy rate): 60 us, of which 3 pass before the first keys are asked for and 6 between the ends of
 // the first and of the last warp's tiles.  48 contexts of 2000 to 6000, 32 / 8 heads, int8 (395 MB, 60 us): 66 us in bursts, 69 to
-// 73, by the GPU, when the power cap has taken the clock to 1.85 or 1.75 GHz.  What else was tried on these two, when they took 61 and
+// 74, by the GPU, when the power cap has taken the clock to 1.85 or 1.75 GHz.  What else was tried on these two, when they took 61 and
 // 70:
 //   80, 90   each lane loads its fragments from global memory into registers, three CTAs of four warps per SM
 //   72, 77   a fifth warp brings the tiles of the four, sixteen copies a turn from four lanes
