@@ -257,10 +257,10 @@ struct PqSums {
       for (int x = 0; x < 2; ++x) {
         const int head = n * 8 + 2 * t + x;
         if (head >= G) continue;
-        const float f = l[n][x] == 0.f ? 0.f : unit * rcp_approx(l[n][x]);
+        const float f = l[n][x] == 0.f ? 0.f : rcp_approx(l[n][x]);            // a small unit times that may be no normal number
         uint32_t r[JT];
 #pragma unroll
-        for (int j = 0; j < JT; ++j) r[j] = pack_bf16x2(acc[n][j][x] * f, acc[n][j][2 + x] * f);
+        for (int j = 0; j < JT; ++j) r[j] = pack_bf16x2(acc[n][j][x] * f * unit, acc[n][j][2 + x] * f * unit);
         pq_put<JT * 4>(o + head * HD + g * (HD / 8), r);
       }
   }
@@ -703,8 +703,10 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             for (int n = 0; n < NT; ++n) pq_mma(acc[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
           }
       };
-      // The unit follows the scales when a ratio leaves [1/2, 64], so that weights keep their fp16 precision and range whatever
-      // the scales of a sequence's blocks are.
+      // The unit follows the scales when a ratio leaves [1/2, 64], so that weights keep their fp16 precision and range whatever the
+      // scales of a sequence's blocks are.  It falls no further than the sums bear: a block of zeros has the least scale there is,
+      // and one after the other they would take any sum out of fp32's range.  Beside sums of 2^118 units or more what is less than
+      // 1/2 of a unit may be rounded away.
       if (unit == 0.f) {
         unit = vs[0] != 0.f ? vs[0] : vs[1];
         per_unit = unit != 0.f ? rcp_approx(unit) : 0.f;
@@ -712,14 +714,23 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (!(vs[u] >= 0.5f * unit && vs[u] <= 64.f * unit) && vs[u] != 0.f) {
-          const float f = fminf(unit * rcp_approx(vs[u]), 0x1p80f);        // beside sums that large a weight is nothing
+          float largest = 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) largest = fmaxf(largest, fabsf(acc[n][j][x]));       // not what is no number
+          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+          const int room = min(max(245 - static_cast<int>(top >> 23), 0), 126);                // sums stay below 2^119
+          const float most = q8_pow2(room), f = fminf(unit * rcp_approx(vs[u]), most);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < JT; ++j)
 #pragma unroll
               for (int x = 0; x < 4; ++x) acc[n][j][x] *= f;
-          unit = f < 0x1p80f ? vs[u] : unit * 0x1p-80f;
+          unit = f < most || top == 0 ? vs[u] : unit * q8_pow2(-room);
           per_unit = rcp_approx(unit);
         }
         add(u);
