@@ -48,6 +48,11 @@ __device__ __forceinline__ bool q8_index_ok(long long i, long long n, int* statu
   return true;
 }
 
+// Whether a slot, negative ones too, lies in the block of `size` tokens whose first slot is `first`, a multiple of size below 2^31.
+__device__ __forceinline__ bool q8_in_block(int slot, int first, int size) {
+  return static_cast<uint32_t>(slot) - static_cast<uint32_t>(first) < static_cast<uint32_t>(size);
+}
+
 __device__ __forceinline__ float q8_pow2(int e) { return __int_as_float((e + 127) << 23); }      // -126 <= e <= 127
 
 // Exponent of the least power of two s with amax <= MAX * s (448 = 1.75 * 2^8, 127 = 1.984375 * 2^6), from the bits of a

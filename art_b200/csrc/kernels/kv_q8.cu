@@ -24,6 +24,7 @@ namespace artb {
 // are under way at a time; runs longer than that are read twice.  (14,000 rows in blocks of 32: 17.7 us, 19.1 with 16 rows of 32 in
 // registers at a time.  Shared memory for runs of 16 too takes 0.8 us more than registers, of 11.8: 14,760 rows in blocks of 16.)
 constexpr int KW_FIT = 32;
+constexpr int KW_STEP = 256;             // rows of a call whose warps take a row each
 template <int KIND, int HD>
 struct KwRun {
   static constexpr int LPR = HD / 8, RPI = 32 / LPR, STEP = 16 / RPI;     // pieces of a lane per 16 rows
@@ -170,13 +171,42 @@ kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int
       asm volatile("prefetch.global.L2 [%0];" ::"l"(x + static_cast<size_t>(row0 + lane / LINES) * ld + lane % LINES * 64));
   }
   const int s = row0 + lane < M ? slot[row0 + lane] : -1;
+  int above = row0 > 0 ? slot[row0 - 1] : -1, seen[ROWS == 1 ? KW_STEP / 32 : 1];
+  if (ROWS == 1) {             // all rows above, on their way together
+#pragma unroll
+    for (int i = 0; i < KW_STEP / 32; ++i) seen[i] = i * 32 + lane < row0 ? slot[i * 32 + lane] : -1;
+  }
   int prev = __shfl_up_sync(0xffffffffu, s, 1);
-  if (lane == 0) prev = row0 > 0 ? slot[row0 - 1] : -1;
+  if (lane == 0) prev = above;
   const int blk = s < 0 ? 0 : block_shift >= 0 ? s >> block_shift : s / block_size;
   const bool goes_on = s > 0 && prev == s - 1 && s != blk * block_size;        // with the run of the row before
-  const uint32_t on = __ballot_sync(0xffffffffu, goes_on);
-  // a second run in the block of the row before would be a second warp's at the same scale: refused
-  const bool astray = s >= 0 && !goes_on && prev >= blk * block_size && prev - blk * block_size < block_size;
+  const uint32_t on = __ballot_sync(0xffffffffu, goes_on), written = __ballot_sync(0xffffffffu, s >= 0);
+  // A second run in a block would be a second warp's at the same scale: refused where it follows the first, rows that are not
+  // written between them or not, and behind any other rows where the call is a step's (0.1 us of 2.7: 256 rows of 4 heads).
+  bool astray;
+  if (ROWS == 1) {
+    const int first = __shfl_sync(0xffffffffu, blk, 0) * block_size;
+    bool again = false;
+#pragma unroll
+    for (int i = 0; i < KW_STEP / 32; ++i) again |= q8_in_block(seen[i], first, block_size);
+    astray = __any_sync(0xffffffffu, again) && s >= 0 && !goes_on;
+  } else {
+    if (above < 0 && (written & ((1u << ROWS) - 1)))
+#pragma unroll 1
+      for (int r = row0 - 2; r >= 0 && above < 0; r -= 256) {
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = r - i * 32 >= lane ? slot[r - i * 32 - lane] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t found = __ballot_sync(0xffffffffu, v[i] >= 0);
+          if (found && above < 0) above = __shfl_sync(0xffffffffu, v[i], __ffs(found) - 1);
+        }
+      }
+    const uint32_t before = written & ((1u << lane) - 1u);
+    const int near = __shfl_sync(0xffffffffu, s, before ? 31 - __clz(before) : 0);
+    astray = s >= 0 && !goes_on && q8_in_block(before ? near : above, blk * block_size, block_size);
+  }
   if (astray && lane < ROWS && status) atomicMax(status, ST_BAD_ARGS);
   // of a team, a run of 17 rows or more is all warps', one of fewer is one warp's
   const bool whose = TEAM == 1 || (lane & 3) == static_cast<int>(threadIdx.x >> 5) || (on >> lane >> 1 & 0xffffu) == 0xffffu;
@@ -267,7 +297,9 @@ kv_rows_q8_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
 using namespace artb;
 
 // slot: block * block_size + place, < 0: the row is not written.
-// A slot beyond the cache is not written either and reported through `status`.
+// A slot beyond the cache is not written either and reported through `status`.  Runs of one block with rows of others between them are
+// refused in calls of up to KW_STEP rows; in longer ones, where finding them would take a look at all rows for each run, they are
+// written at the same time and what the block then holds is undefined.
 ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
   const int M = a->n, ld = a->ld, Hkv = a->Hkv, hd = a->hd, block_size = a->block_size, kind = a->kind;
   if (M <= 0) return 0;
@@ -283,7 +315,7 @@ ARTB_EXPORT int artb_kv_write_q8(const KvRowsArgs* a, cudaStream_t st) {
                                             (uint8_t*)a->k_cache, (uint8_t*)a->v_cache, a->k_scale, a->v_scale, M, Hkv,      \
                                             block_size, shift, a->num_blocks, a->status));                                   \
     };                                                                                                                       \
-    if (M <= 256) return go(kv_write_q8_kernel<KIND_, HD_, 1, 1>, 1, 4);                                                     \
+    if (M <= KW_STEP) return go(kv_write_q8_kernel<KIND_, HD_, 1, 1>, 1, 4);                                                    \
     if (block_size > 32) return go(kv_write_q8_kernel<KIND_, HD_, 16, 4>, 16, 1);                                            \
     if (M <= 2048) return go(kv_write_q8_kernel<KIND_, HD_, 4, 1>, 4, 4);                                                    \
     return go(kv_write_q8_kernel<KIND_, HD_, 16, 1>, 16, 4);                                                                 \

@@ -138,8 +138,10 @@ def kv_write_q8(qkv: torch.Tensor, k_col: int, v_col: int, slot: torch.Tensor, k
                 k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
     """Quantises the keys and values of the rows of ``qkv`` (bf16 [M, >= ...], columns ``k_col`` and ``v_col`` on) into the cache.
     ``slot`` int32 [M]: block * block_size + place, negative: the row is not written.  The rows that go to one block are neighbours and
-    go to consecutive places, as those of a prompt and of a decode step do; a row that follows one of its block elsewhere is not
-    written and reported through the status word, as are slots beyond the cache.
+    go to consecutive places, as those of a prompt and of a decode step do.  A row that comes behind others of its block and is not
+    their neighbour at the next place, rows that are not written between them or not, is not written and reported through the status
+    word, as are slots beyond the cache.  Calls of up to 256 rows report it of blocks that take turns (5, 40, 6 in blocks of 16) too;
+    in longer calls such blocks are not found, and what they then hold is undefined.
 
     The scale of a block and head is the least power of two that takes the largest value written to it into the range of the
     codes.  A row at a block's first place starts the block anew.  Rows at later places can only raise the scale, and then what
