@@ -224,12 +224,12 @@ decode_finalize_norm_kernel(float* __restrict__ ws, int ldw, int N, int kpad, co
 // pass; 64 such rows with 24 low-rank columns took 19 us in two passes and take 11.  Beyond, two CTAs of 256 threads (128
 // registers) per SM: with 320, which make 28 / 4 heads one pass, registers spill (256 rows: 16 -> 19 us).
 //
-// KIND >= 0: the cache is held in 8 bits (kv_q8.cuh), and no two rows of a launch belong to one block.  The lanes that hold a head
-// then agree on its largest value; keys and values are rounded to bf16 first, as the bf16 cache would hold them.  Old scales are
-// read ahead, and blocks whose scale was raised are rounded to it at the end by the whole CTA: one of every ten or so heads of a
-// step is, and eight lanes that did it by themselves held up the launch (6.99 ms a step of 256 sequences of qwen2.5-7b, 6.81 so).
-// Beside a launch of its own for the write: 4.43 ms a step instead of 4.47 (64 sequences of qwen2.5-7b), 6.45 instead of 6.56 (128
-// of qwen3-8b), 6.81 instead of 6.87 (256 of qwen2.5-7b).
+// KIND >= 0: the cache is held in 8 bits (kv_q8.cuh), and no two rows of a launch belong to one block (the later of such two is not
+// written and reported).  The lanes that hold a head then agree on its largest value; keys and values are rounded to bf16 first, as the
+// bf16 cache would hold them.  Old scales are read ahead, and blocks whose scale was raised are rounded to it at the end by the whole
+// CTA: one of every ten or so heads of a step is, and eight lanes that did it by themselves held up the launch (6.99 ms a step of 256
+// sequences of qwen2.5-7b, 6.81 so).  Beside a launch of its own for the write: 4.43 ms a step instead of 4.47 (64 sequences of
+// qwen2.5-7b), 6.45 instead of 6.56 (128 of qwen3-8b), 6.81 instead of 6.87 (256 of qwen2.5-7b).
 constexpr int DQ_BF16 = -1;
 
 constexpr int DQ_HEADS = 256;        // keys' and values' heads of a cache in 8 bits together
@@ -297,6 +297,12 @@ decode_finalize_qkv_kernel(float* __restrict__ ws, int ldw, int Hq, int Hkv, int
   if (s >= 0 && !(KIND == DQ_BF16 ? index_ok(s, num_slots, status) : q8_index_ok(s, num_slots, status))) s = -1;   // reported, not written
   const int block = KIND == DQ_BF16 || s < 0 ? 0 : s / q8.block_size, at = KIND == DQ_BF16 || s < 0 ? 0 : s - block * q8.block_size;
   if constexpr (KIND != DQ_BF16) {
+    bool again = false;                // a row above belongs to the block: this one would change its scale at the same time
+    for (int i = threadIdx.x; i < row; i += DQ_THREADS) again |= q8_in_block(slot[i], block * q8.block_size, q8.block_size);
+    if (__syncthreads_or(again) && s >= 0) {                     // 0.3 us of 17 (256 rows of 28 / 4 heads)
+      if (threadIdx.x == 0 && status) atomicMax(status, ST_BAD_ARGS);
+      s = -1;
+    }
     if (s >= 0 && static_cast<int>(threadIdx.x) < 2 * Hkv) {
       const int h = threadIdx.x < Hkv ? threadIdx.x : threadIdx.x - Hkv;
       held_s[threadIdx.x] = __ldcg((static_cast<int>(threadIdx.x) < Hkv ? q8.k_scale : q8.v_scale) + static_cast<size_t>(block) * Hkv + h);
@@ -461,7 +467,8 @@ ARTB_EXPORT int artb_decode_finalize_qkv(float* ws, int ldw, int M, int Hq, int 
 }
 
 // The same into a cache in 8 bits (codes [num_blocks, Hkv, block_size, hd], scales [num_blocks, Hkv]): no two of the M slots lie in one
-// block.  hd 32, 64 or 128 and an even number of q and k heads together, so that a head's values lie in neighbouring lanes.
+// block (the later row of such two is not written and reported through `status`).  hd 32, 64 or 128 and an even number of q and k heads
+// together, so that a head's values lie in neighbouring lanes.
 ARTB_EXPORT int artb_decode_finalize_qkv_q8(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int kpad, const float* bias,
                                             const int* adapter, const void* B_all, int ldb, int cols, const int* pos,
                                             float theta, const void* q_norm, const void* k_norm, float eps, const int* slot,

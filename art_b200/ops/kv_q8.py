@@ -162,8 +162,8 @@ def decode_finalize_qkv_q8(ws: torch.Tensor, M: int, Hq: int, Hkv: int, hd: int,
                            adapter: torch.Tensor | None = None, B_all: torch.Tensor | None = None, cols: int = 0,
                            q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> None:
     """:func:`~art_b200.ops.paged.decode_finalize_qkv` into a cache in 8 bits, the same numbers as that and :func:`kv_write_q8` of
-    its bf16 rows in one launch.  No two of the ``M`` slots lie in one block: the rows are those of a decode step.  ``Hq + Hkv`` is
-    even (:func:`finalize_covers`)."""
+    its bf16 rows in one launch.  No two of the ``M`` slots lie in one block, as in a decode step: the later row of
+    such two is not written and reported through the status word.  ``Hq + Hkv`` is even (:func:`finalize_covers`)."""
     nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
     if hkv != Hkv or d != hd or not finalize_covers(Hq, Hkv):
         raise ValueError(f"{Hq} query heads and {Hkv} kv heads of {hd}: the cache has {hkv} of {d}, and the number of both must be even")

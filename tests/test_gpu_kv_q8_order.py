@@ -101,3 +101,31 @@ def test_rows_above_in_no_block():
         for j in range(2):
             o[j].write(x[:, j * Hkv * hd:(j + 1) * Hkv * hd], [s if 0 <= s < 64 else -1 for s in slots])
         same(cache, *o)
+
+
+@KINDS
+@pytest.mark.parametrize("rows,twice", [(3, {2: 0}), (9, {3: 1, 8: 1, 6: 4}), (300, {299: 0, 270: 250, 256: 255})])
+def test_finish(dtype, rows, twice):
+    """Of two rows of one block the later is not written and reported; its query is there, and so are all others."""
+    from art_b200.ops import _lib, kv_q8
+
+    Hq, Hkv, hd, bs = 4, 2, 64, 32
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    ws = torch.randn(rows, (Hq + 2 * Hkv) * hd, generator=g, device=DEV)
+    pos = torch.randint(0, 500, (rows,), generator=g, device=DEV).int()
+    slot = torch.randperm(rows + 2, generator=g, device=DEV)[:rows].int() * bs + torch.randint(0, bs, (rows,), generator=g, device=DEV).int()
+    slot[rows // 2] = -1
+    want = slot.clone()
+    for later, first in twice.items():
+        slot[later], want[later] = slot[first] // bs * bs + (slot[first] + 7) % bs, -1
+    results = []
+    for s in (slot, want):
+        cache, q = filled(rows + 2, Hkv, bs, hd, dtype, torch.Generator(device=DEV).manual_seed(1)), torch.zeros(rows, Hq * hd, dtype=torch.bfloat16, device=DEV)
+        kv_q8.decode_finalize_qkv_q8(ws.clone(), rows, Hq, Hkv, hd, 0, pos, 1e6, s, *cache, q)
+        if s is slot:
+            with pytest.raises(_lib.KernelStatusError):
+                _lib.check_status()
+        else:
+            _lib.check_status()
+        results.append([q, *(c.double() for c in cache)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
