@@ -18,13 +18,26 @@ class UnsupportedPrecision(ValueError):
     """The model family does not run in the requested number format."""
 
 
+def cache_dtype(cfg, block_size: int, name: str | torch.dtype | None) -> torch.dtype:
+    """The number format ``name`` (``kv_cache.KV_CACHE_DTYPES``; None: that of the model) for a cache of ``cfg``; ValueError where the
+    model's caches are not held in it."""
+    dtype = kv_cache_dtype(name)
+    if dtype != torch.bfloat16:
+        from ..ops.kv_q8 import check_geometry
+
+        if isinstance(cfg, HybridConfig):
+            raise ValueError("hybrid models keep their caches in the model's number format")
+        check_geometry(dtype, block_size, cfg.head_dim, cfg.num_heads // cfg.num_kv_heads)
+    return dtype
+
+
 def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, block_size: int = 16, num_slots: int = 256,
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, lora_cfg: LoraConfig | None = None,
                  max_loras: int = 4, tp_group=None, decoder=None, use_arena: bool = False,
                  kv_dtype: str | torch.dtype | None = None):
     """``(runner, cache)`` on ``device``.  ``num_slots`` bounds the sequences that hold recurrent state at once.  ``kv_dtype``: the
     cache's number format (``kv_cache.KV_CACHE_DTYPES``; None: that of the model)."""
-    cache_dtype = kv_cache_dtype(kv_dtype)
+    kv_dtype = cache_dtype(cfg, block_size, kv_dtype)
     dev = torch.device(device)
     if dev.type == "cuda" and dev.index is None:       # the engine's stepping thread selects it by number
         dev = torch.device("cuda", torch.cuda.current_device())
@@ -33,8 +46,6 @@ def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, 
 
         if tp_group is not None and torch.distributed.get_world_size(tp_group) > 1:
             raise ValueError("hybrid models run on one GPU per replica")
-        if cache_dtype != torch.bfloat16:
-            raise ValueError("hybrid models keep their caches in the model's number format")
         kv = HybridCache(cfg, num_blocks, block_size, num_slots, dev, dtype)
         return HybridRunner(cfg, kv, base, device=dev, dtype=dtype), kv
     from .runner import NativeRunner
@@ -42,7 +53,7 @@ def build_runner(cfg, base: dict[str, torch.Tensor] | None, *, num_blocks: int, 
     if dtype != torch.bfloat16:
         raise UnsupportedPrecision(f"{cfg.family} models run in bfloat16")
     tp = 1 if tp_group is None else torch.distributed.get_world_size(tp_group)
-    args = (cfg.num_layers, num_blocks, block_size, cfg.num_kv_heads // tp, cfg.head_dim, dev, cache_dtype)
+    args = (cfg.num_layers, num_blocks, block_size, cfg.num_kv_heads // tp, cfg.head_dim, dev, kv_dtype)
     try:
         kv = KVCache(*args, use_arena=use_arena)
     except RuntimeError:   # no VMM support: plain tensors; Engine.sleep() then drops the captured graphs

@@ -50,14 +50,19 @@ def _f(name: str):
     return fn
 
 
-def check_geometry(dtype: torch.dtype, block_size: int, hd: int) -> None:
-    """Refuses what the kernels do not cover."""
+MOST_HEADS = 16                 # query heads of a kv head
+
+
+def check_geometry(dtype: torch.dtype, block_size: int, hd: int, group: int = 1) -> None:
+    """Refuses what the kernels do not cover; ``group``: query heads of a kv head."""
     if dtype not in KINDS:
         raise ValueError(f"a cache of {dtype}: codes are float8_e4m3fn or int8")
     if block_size < 16 or block_size % 16:
         raise ValueError(f"blocks of {block_size} tokens: a cache in 8 bits has blocks of a multiple of 16")
     if hd not in HEAD_DIMS:
         raise ValueError(f"head dim {hd}: a cache in 8 bits takes {', '.join(map(str, HEAD_DIMS))}")
+    if group > MOST_HEADS:
+        raise ValueError(f"{group} query heads to a kv head: a cache in 8 bits takes at most {MOST_HEADS}")
 
 
 def _check_cache(k_cache, v_cache, k_scale, v_scale) -> None:
@@ -243,8 +248,8 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     :func:`kv_write_q8` leaves them.  Entries that are no block and lengths that the table cannot hold are reported through the
     status word; such keys are left out.  The same inputs give the same bits."""
     nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
-    if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > 16 * Hkv:
-        raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most 16")
+    if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > MOST_HEADS * Hkv:
+        raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most {MOST_HEADS}")
     n, ldq, at = _rows("q", q, 0, 0, Hq * hd)
     m, ldo, to = _rows("out", out, 0, 0, Hq * hd)
     if m != n or ldo < Hq * hd or (abs(to - at) < 2 * n * max(ldq, ldo) and _meet(at, ldq, to, ldo, n, Hq * hd)):
