@@ -177,7 +177,7 @@ def kv_cache_dtype(name: str | torch.dtype | None) -> torch.dtype:
     """The number format of a cache from its name (None: bf16)."""
     if isinstance(name, torch.dtype) and name in KV_CACHE_DTYPES.values():
         return name
-    if name is None or name in KV_CACHE_DTYPES:
+    if name is None or (isinstance(name, str) and name in KV_CACHE_DTYPES):
         return KV_CACHE_DTYPES[name or "auto"]
     raise ValueError(f"kv_cache_dtype {name!r}: supported are {', '.join(KV_CACHE_DTYPES)}")
 

@@ -18,6 +18,7 @@ Contract parity: reference ``src/art/local/service.py:26-174`` (``start_openai_s
 from __future__ import annotations
 
 import asyncio
+import logging
 import os
 import threading
 import time
@@ -36,6 +37,8 @@ from ..utils.output_dirs import get_step_checkpoint_dir
 from .checkpoints import get_last_checkpoint_dir
 from .pack import DiskPackedTensors, packed_tensors_from_dir
 from .tokenizer import load_tokenizer
+
+log = logging.getLogger(__name__)
 
 TRAINER_STATE = "trainer_state.pt"
 
@@ -100,7 +103,8 @@ class ModelState:
     def __init__(self, base_model: str, config: dev.InternalModelConfig, output_dir: str, rank: int = 0, world: int = 1,
                  tp: int = 1, master_port: int = 0):
         from ..engine.engine import Engine
-        from ..engine.kv_cache import BlockManager, kv_cache_dtype
+        from ..engine.factory import cache_dtype
+        from ..engine.kv_cache import BlockManager
         from ..trainer.trainer import Trainer
 
         init_args = config.get("init_args", {})
@@ -197,7 +201,15 @@ class ModelState:
         # rollout engine: one replica per rank
         block_size = int(engine_args.get("block_size") or 16)
         max_loras = int(engine_args.get("max_loras", 4))
-        kv_dtype = kv_cache_dtype(engine_args.get("kv_cache_dtype"))
+        kv_dtype = torch.bfloat16
+        try:
+            kv_dtype = cache_dtype(self.cfg, block_size, engine_args.get("kv_cache_dtype"))
+            if kv_dtype != torch.bfloat16 and self.device.type != "cuda":
+                raise ValueError("models on the CPU keep no cache")
+        except ValueError as e:      # a configuration written for another engine runs all the same
+            kv_dtype = torch.bfloat16
+            if rank == 0:
+                log.warning("engine_args['kv_cache_dtype'] has no effect here: %s", e)
         max_len = int(engine_args.get("max_model_len") or init_args.get("max_seq_length", 32768))
         if self.device.type == "cuda":
             from ..engine.factory import build_runner, cache_bytes
