@@ -393,6 +393,31 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   auto result = [&](int seq) { return out + static_cast<size_t>(seq) * ldo + kvh * G * HD; };
   auto piece_at = [&](int w) { return reinterpret_cast<float*>(rings + PQ_WARPS * S::RING + w * S::PIECE); };
   auto ring_at = [&](int w) { return reinterpret_cast<float*>(rings + w * S::RING); };
+  auto locate = [&](int x, int& seq, int& len) {              // the sequence that tile x is of, and its first tile
+    int a = 0, b = entries;
+#pragma unroll 1
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (s_first[mid] <= x) a = mid;
+      else b = mid;
+    }
+    int first = s_first[a];
+    seq = a * run;
+    len = run == 1 ? s_len[a] : checked(ctx_len[seq]);
+#pragma unroll 1
+    while (x >= first + tiles_in(len) && seq + 1 < nseq) {
+      first += tiles_in(len);
+      len = checked(ctx_len[++seq]);
+    }
+    return first;
+  };
+  // A part of a sequence is there (released with what the thread's warp wrote): number, first share, parts, whether it is the last.
+  auto count_part = [&](int seq, int len, int first) {
+    const int sh0 = first / per, parts = (first + tiles_in(len) - 1) / per - sh0 + 1;
+    int seen;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(&count[seq * Hkv + kvh]) : "memory");
+    return make_int4(seq, sh0, parts, seen == parts - 1);
+  };
   PqSums<NT, JT> sums;
   auto& m = sums.m;
   auto& l = sums.l;
@@ -407,22 +432,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     int blk[2];
     auto find = [&](int i) {                // which it is, and its blocks on their way
       if (lane >= PQ_ROUND || i >= tiles) return;
-      const int x = lo + i;
-      int a = 0, b = entries;
-#pragma unroll 1
-      while (b - a > 1) {
-        const int mid = (a + b) >> 1;
-        if (s_first[mid] <= x) a = mid;
-        else b = mid;
-      }
-      int first = s_first[a];
-      next.seq = a * run;
-      next.len = run == 1 ? s_len[a] : checked(ctx_len[next.seq]);
-#pragma unroll 1
-      while (x >= first + tiles_in(next.len) && next.seq + 1 < nseq) {
-        first += tiles_in(next.len);
-        next.len = checked(ctx_len[++next.seq]);
-      }
+      const int x = lo + i, first = locate(x, next.seq, next.len);
       next.tile = x - first;
       const int left = next.len - next.tile * PQ_KEYS;
       next.keys = min(left, 16) | max(0, min(left - 16, 16)) << 8;
@@ -780,6 +790,15 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __syncthreads();
   if (s_abort) {                              // no copy may outlive the CTA
     if (lane < STAGES) mbar_wait_timed(&s_full[warp][lane], 0, 100), mbar_wait_timed(&s_full[warp][lane], 1, 100);
+    if (tid == 0) {                           // what was computed is lost, but the parts are counted as ever: the next launch finds zeros
+      auto count_lost = [&](int seq, int len, int first) {
+        if (count_part(seq, len, first).w) count[seq * Hkv + kvh] = 0;
+      };
+      int seq, len, first = locate(at, seq, len);
+      if (first < at) count_lost(seq, len, first);
+      first = locate(end - 1, seq, len);
+      if (first >= at && first + tiles_in(len) > end) count_lost(seq, len, first);
+    }
     return;
   }
   bool gives = false;
@@ -806,10 +825,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __syncwarp();
   if (lane == 0 ? middle : lane == 1 && gives && last.lo == 0) {
     const PqPiece piece = lane == 0 && owes ? owed : last;
-    const int sh0 = piece.first / per, parts = (piece.first + tiles_in(piece.len) - 1) / per - sh0 + 1;
-    int seen;                                                  // releases what the warp wrote
-    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(&count[piece.seq * Hkv + kvh]) : "memory");
-    if (seen == parts - 1) s_part[lane] = make_int4(piece.seq, sh0, parts, 1);
+    const int4 counted = count_part(piece.seq, piece.len, piece.first);
+    if (counted.w) s_part[lane] = counted;
   }
   __syncthreads();
 #pragma unroll 1
@@ -881,8 +898,9 @@ static int pq_map(CUtensorMap* map, const void* codes, long rows, int hd) {
 
 using namespace artb;
 
-// Bytes of workspace: two parts per CTA, then counters [num_seqs * Hkv] (zero before the first call, zero again after each).  The
-// counters lie behind what does not depend on the batch, so that a call with fewer sequences leaves those of a larger one alone.
+// Bytes of workspace: two parts per CTA, then counters [num_seqs * Hkv] (zero before the first call, zero again after each, one whose
+// waits ran out too).  The counters lie behind what does not depend on the batch, so that a call with fewer sequences leaves those of a
+// larger one alone.
 ARTB_EXPORT int artb_paged_decode_q8_bytes(int num_seqs, int Hq, int Hkv, int hd) {
   if (num_seqs <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 16) return 0;
   return static_cast<int>(pq_part_bytes(Hq, Hkv, hd) + (static_cast<long>(num_seqs) * Hkv + 3) / 4 * 16);
