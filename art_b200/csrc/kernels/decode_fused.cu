@@ -446,7 +446,11 @@ static int finalize_qkv(float* ws, int ldw, int M, int Hq, int Hkv, int hd, int 
   if ((hd & 15) || hd > 256 || (ldw & 3) || (ldq & 7) || Hq <= 0 || Hkv <= 0 || !pos || !slot) return ERR_BAD_SHAPE;
   if (!q_norm != !k_norm || (q_norm && (hd & (hd - 1)))) return ERR_BAD_SHAPE;
   if (adapter && (cols <= 0 || cols > DF_MAX_COLS || (kpad & 3) || (ldb & 7) || !B_all)) return ERR_BAD_SHAPE;
-  if (reinterpret_cast<uintptr_t>(ws) & 15) return ERR_BAD_ALIGN;
+  uintptr_t bits = 0;
+  for (const void* p : {static_cast<const void*>(ws), static_cast<const void*>(bias), adapter ? B_all : nullptr, q_norm, k_norm,
+                        static_cast<const void*>(k_cache), static_cast<const void*>(v_cache), static_cast<const void*>(q_out)})
+    bits |= reinterpret_cast<uintptr_t>(p);
+  if (bits & 15) return ERR_BAD_ALIGN;
   auto go = [&](auto kern, int threads) {
     return static_cast<int>(launch_kernel(
         kern, dim3(M), dim3(threads), 0, st, ws, ldw, Hq, Hkv, hd, kpad, bias, adapter,
