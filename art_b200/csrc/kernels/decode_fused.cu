@@ -228,8 +228,8 @@ decode_finalize_norm_kernel(float* __restrict__ ws, int ldw, int N, int kpad, co
 // written and reported).  The lanes that hold a head then agree on its largest value; keys and values are rounded to bf16 first, as the
 // bf16 cache would hold them.  Old scales are read ahead, and blocks whose scale was raised are rounded to it at the end by the whole
 // CTA: one of every ten or so heads of a step is, and eight lanes that did it by themselves held up the launch (6.99 ms a step of 256
-// sequences of qwen2.5-7b, 6.81 so).  Beside a launch of its own for the write: 4.43 ms a step instead of 4.47 (64 sequences of
-// qwen2.5-7b), 6.45 instead of 6.56 (128 of qwen3-8b), 6.81 instead of 6.87 (256 of qwen2.5-7b).
+// sequences of qwen2.5-7b, 6.81 so).  Beside a launch of its own for the write: 4.36 ms a step and 4.35 (64 sequences of qwen2.5-7b),
+// 6.40 and 6.54 (128 of qwen3-8b), 6.58 and 6.63 (256 of qwen2.5-7b).
 constexpr int DQ_BF16 = -1;
 
 constexpr int DQ_HEADS = 256;        // keys' and values' heads of a cache in 8 bits together

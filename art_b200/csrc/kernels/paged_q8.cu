@@ -715,8 +715,8 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       };
       // The unit follows the scales when a ratio leaves [1/2, 64], so that weights keep their fp16 precision and range whatever the
       // scales of a sequence's blocks are.  It falls no further than the sums bear: a block of zeros has the least scale there is,
-      // and one after the other they would take any sum out of fp32's range.  Beside sums of 2^118 units or more what is less than
-      // 1/2 of a unit may be rounded away.
+      // and one after the other they would take any sum out of fp32's range.  Beside sums of 2^118 units or more the weights of
+      // smaller blocks are rounded to 2^-25 units.
       if (unit == 0.f) {
         unit = vs[0] != 0.f ? vs[0] : vs[1];
         per_unit = unit != 0.f ? rcp_approx(unit) : 0.f;

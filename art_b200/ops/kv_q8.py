@@ -245,8 +245,9 @@ def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     ws: torch.Tensor) -> torch.Tensor:
     """Attention of one token per sequence over the first ``ctx_len`` cached tokens: q bf16 [n, >= Hq*hd] (row stride arbitrary),
     ``block_table`` int32 [n, width], ``ctx_len`` int32 [n] (0: the row becomes zeros); out bf16 [n, >= Hq*hd].  Scales are as
-    :func:`kv_write_q8` leaves them.  Entries that are no block and lengths that the table cannot hold are reported through the
-    status word; such keys are left out.  The same inputs give the same bits."""
+    :func:`kv_write_q8` leaves them.  Values of 2^120 / ``ctx_len`` and more may overflow the fp32 sums.  Entries that are no block
+    and lengths that the table cannot hold are reported through the status word; such keys are left out.  The same inputs give the
+    same bits."""
     nb, hkv, bs, d, kind = _geometry(k_cache, v_cache, k_scale, v_scale)
     if hkv != Hkv or d != hd or Hq <= 0 or Hq % Hkv or Hq > MOST_HEADS * Hkv:
         raise ValueError(f"{Hq} query heads of {hd} over {Hkv} kv heads: the cache has {hkv} of {d}, and a kv head serves at most {MOST_HEADS}")
