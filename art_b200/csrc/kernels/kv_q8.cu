@@ -141,11 +141,12 @@ struct KwRun {
   }
 };
 
-// ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 3.3 us, 4.6 with four to a warp, 12 with
-// sixteen), a block's worth where prompts bring many (14,000 rows, when that was 20 us: 26 with four to a warp, 64 with one).
+// ROWS: a row per warp where a step's sequences bring one each (256 rows of 8 heads of 128: 4.1 us, 4.4 with four to a warp, 11.6 with
+// sixteen; of 4 heads 2.7, 4.1 and 11.4), a block's worth where prompts bring many (14,000 rows, when that was 20 us: 26 with four to a
+// warp, 64 with one).
 // TEAM: of blocks of more than 32 rows a run is four warps', which find the same runs and share the rows of a long one (1000 rows in
-// blocks of 64: 4.5 us, 8.1 with a warp to each; 8192 in blocks of 128: 17.7 and 23.6; but 512 rows in as many blocks 6.3 and 5.2, and
-// 2000 rows in blocks of 32 7.6 and 6.9).
+// blocks of 64: 3.5 us, 7.1 with a warp to each; 8192 in blocks of 128: 17.1 and 23.3; but 512 rows in as many blocks 6.2 and 5.4, and
+// 2000 rows in blocks of 32 6.9 and 5.0).
 template <int KIND, int HD, int ROWS, int TEAM>
 __global__ void __launch_bounds__(128, ROWS == 1 ? 8 : 7)
 kv_write_q8_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int k_col, int v_col, const int* __restrict__ slot,
